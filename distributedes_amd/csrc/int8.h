@@ -1,0 +1,94 @@
+// 8-bit rows: what the quantising and the product kernels share.
+//
+// A row x of K values is held as codes q in [-127, 127] and one fp32 scale s:
+//     a = max |x_k|,  s = max(fp32(a / 127), 2^-126),
+//     q_k = the whole number nearest to x_k / s, ties to even.
+// The quotient is the exact one: codes do not depend on how a division rounds,
+// so kernel, torch twin and a 64-bit oracle agree bit for bit.  The bound
+// 2^-126 keeps the scale of rows of zeros (and of values below any use) a
+// normal number, so that nothing divides by zero.  A row that holds a NaN or an
+// infinity gets scale NaN and codes 0: it shows in every product.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace des {
+
+// element types of float rows and of results, as the bindings pass them
+enum Elem : int { ELEM_F32 = 0, ELEM_BF16 = 1, ELEM_F16 = 2 };
+
+struct Bf16 { uint16_t bits; };
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(_Float16 v) { return (float)v; }
+__device__ __forceinline__ float to_f32(Bf16 v) {
+  return __uint_as_float((uint32_t)v.bits << 16);
+}
+
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) {
+  return v;
+}
+template <> __device__ __forceinline__ _Float16 from_f32<_Float16>(float v) {
+  return (_Float16)v;
+}
+// to nearest, ties to even; a NaN stays one (adding the half step could carry
+// its mantissa over into an infinity)
+template <> __device__ __forceinline__ Bf16 from_f32<Bf16>(float v) {
+  uint32_t b = __float_as_uint(v);
+  if ((b & 0x7FFFFFFFu) > 0x7F800000u) return Bf16{(uint16_t)0x7FC0};
+  return Bf16{(uint16_t)((b + 0x7FFFu + ((b >> 16) & 1u)) >> 16)};
+}
+
+// |v| as bits: among floats these order like the values, infinity and NaN above
+// all others, so one unsigned maximum finds both the largest and the unusable
+__device__ __forceinline__ uint32_t abs_bits(float v) {
+  return __float_as_uint(v) & 0x7FFFFFFFu;
+}
+
+struct RowScale {
+  float scale, inv;  // inv = 0 where the row is unusable
+};
+
+__device__ __forceinline__ RowScale row_scale(uint32_t top) {
+  RowScale r;
+  if (top >= 0x7F800000u) {
+    r.scale = __uint_as_float(0x7FC00000u);
+    r.inv = 0.f;
+  } else {
+    r.scale = fmaxf(__uint_as_float(top) / 127.0f, 1.17549435e-38f);
+    r.inv = 1.0f / r.scale;
+  }
+  return r;
+}
+
+// The code of v.  rint(v * inv) is at most one step off, and only next to a
+// border; the remainder v - q s has at most 24 bits there, so the fma is exact
+// and tells on which side of the border (or on it) v lies.
+__device__ __forceinline__ int row_code(float v, RowScale r) {
+  float q = rintf(v * r.inv);
+  float rem = fmaf(-q, r.scale, v);
+  float twice = 2.0f * fabsf(rem);
+  if (twice >= r.scale && r.inv != 0.f) {
+    if (twice > r.scale || ((int)q & 1)) q += rem > 0.f ? 1.0f : -1.0f;
+  }
+  return r.inv == 0.f ? 0 : (int)q;
+}
+
+}  // namespace des
+
+// One batch of products, as the bindings pass it.  Strides in elements; the
+// elements of a row are next to each other.
+struct DesInt8Product {
+  const int8_t* x;      // [B, M, K]
+  const float* sx;      // [B, M]
+  const int8_t* w;      // [B, N, K]
+  const float* sw;      // [B, N]
+  const float* bias;    // nullable [B, N]
+  void* y;              // [B, M, N]
+  int64_t B;
+  int32_t M, N, K;
+  int64_t xsb, xsr, wsb, wsr;
+  int32_t act;          // 0 none, 1 relu, 2 tanh
+  int32_t out;          // des::Elem
+};

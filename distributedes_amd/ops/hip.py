@@ -1,7 +1,8 @@
-"""HIP kernel backend: loads the in-tree gfx950 extension.
+"""HIP kernel backend: loads the in-tree gfx950 extensions.
 
-The extension is built IN-TREE (setup.py build_ext --inplace -> _hip_ops.so
-next to this file) so the .so ships with the repo snapshot to GPU boxes.
+The extensions are built IN-TREE (setup.py build_ext --inplace -> _hip_ops.so
+and _hip_ops2.so next to this file) so the .so ship with the repo snapshot to
+GPU boxes.
 On a GPU box, ops FAIL LOUDLY if the extension is missing — no silent
 eager fallback (the engine enforces this in _make_ops).
 """
@@ -12,18 +13,21 @@ import importlib
 import torch
 
 _ext = None
+_ext2 = None
 _err = None
 
 
 def _load():
-    global _ext, _err
+    global _ext, _ext2, _err
     if _ext is not None or _err is not None:
         return _ext
     try:
-        from . import _hip_ops  # built in-tree
-        _ext = _hip_ops
+        # built in-tree; _hip_ops2: 8-bit rows and products, gradient norm
+        from . import _hip_ops, _hip_ops2
+        _ext, _ext2 = _hip_ops, _hip_ops2
     except ImportError as e:
         try:
+            _ext2 = importlib.import_module("_hip_ops2")
             _ext = importlib.import_module("_hip_ops")
         except ImportError:
             _err = e
@@ -46,6 +50,7 @@ class HipOps:
 
     def __init__(self):
         self.ext = _load()
+        self.ext2 = _ext2
         if self.ext is None:
             raise RuntimeError(f"HIP extension not built: {_err}")
 
@@ -82,3 +87,52 @@ class HipOps:
         self.ext.weighted_noise_sum(acc, acc_sq, table, offsets, signs,
                                     weights, bool(want_sq))
         return (acc, acc_sq) if want_sq else acc
+
+    # --- 8-bit rows and products -----------------------------------------
+    # No gradient passes through these: the framework estimates its gradients
+    # from forward passes.  An argument that requires one is refused.
+
+    def quantize_rows(self, x, out=None):
+        """x [..., K] (fp32/bf16/fp16, K <= 131072) -> (codes [..., K] int8,
+        scale [...] fp32), with x ~ codes * scale: one scale a row,
+        max(fp32(max|x| / 127), 2^-126), and codes the whole numbers nearest
+        to x / scale, ties to even.  A row that holds a NaN or an infinity
+        gets scale NaN and codes 0.
+
+        Fresh codes are a view whose rows begin at multiples of 16 bytes.
+        out: (codes, scale) to write to; the codes' rows may lie anywhere
+        apart from one another (bytes between them are left as they were)."""
+        q, s = out if out is not None else (None, None)
+        return self.ext2.quantize_rows(x, q, s)
+
+    def int8_matmul(self, xq, sx, wq, sw, bias=None, activation="none",
+                    out_dtype=torch.float32, out=None):
+        """act(sum_k xq[m, k] wq[n, k] * sx[m] * sw[n] + bias[n]): codes and
+        scales of quantize_rows on both sides, summed exactly in int32.
+
+        One policy: xq [..., K] with wq [N, K] -> [..., N].  Members with
+        weights of their own: xq [B, M, K] with wq [B, N, K] -> [B, M, N].
+        sx, sw, bias: fp32, shaped like the rows they belong to.
+        activation: none | relu | tanh.  out_dtype: fp32 | bf16 | fp16.
+        out: a contiguous tensor to write to."""
+        return self.ext2.int8_matmul(xq, sx, wq, sw, bias, activation,
+                                     out_dtype, out)
+
+    def int8_linear(self, x, wq, sw, bias=None, activation="none",
+                    out_dtype=torch.float32, out=None):
+        """int8_matmul of quantize_rows(x): x fp32/bf16/fp16."""
+        return self.ext2.int8_linear(x, wq, sw, bias, activation, out_dtype,
+                                     out)
+
+    # --- gradient norm ----------------------------------------------------
+    def global_norm(self, tensors):
+        """sqrt of the sum of squares over all tensors (fp32/bf16/fp16, mixed
+        as they come), summed in fp64 -> fp32 scalar tensor."""
+        return self.ext2.global_norm(tensors)
+
+    def clip_by_global_norm(self, tensors, max_norm, out=None):
+        """-> ([t * c for t in tensors], norm), with c = max_norm / norm (fp64)
+        where norm > max_norm, else 1; the norm stays on the GPU.  A NaN norm
+        leaves the values as they are, an infinite one gives c = 0.
+        out: tensors to write to (the tensors themselves clip in place)."""
+        return self.ext2.clip_by_global_norm(tensors, max_norm, out)

@@ -11,6 +11,37 @@ import torch
 
 from ..core import noise as noise_mod
 
+_MAX_COLS = 131072     # int32 sums of 127 * 127 stay in range
+_ELEMS = (torch.float32, torch.bfloat16, torch.float16)
+_ACTS = ("none", "relu", "tanh")
+
+
+def _want(ok, message):
+    if not ok:
+        raise ValueError(message)
+
+
+def _want_product(x, wq, sw, bias, activation, out_dtype, out):
+    _want(wq.dtype == torch.int8, "wq must be int8")
+    _want(wq.dim() in (2, 3),
+          "wq must be [channels, cols] or [members, channels, cols]")
+    _want(wq.dim() == 2 or x.dim() == 3,
+          "members' weights need x of [members, tokens, cols]")
+    _want(x.shape[-1] == wq.shape[-1], "x and wq differ in cols")
+    _want(wq.dim() == 2 or x.shape[0] == wq.shape[0],
+          "x and wq differ in members")
+    _want(x.shape[-1] <= _MAX_COLS, f"rows of at most {_MAX_COLS} values")
+    _want(sw.dtype == torch.float32 and sw.shape == wq.shape[:-1],
+          "sw must be float32 of wq's shape without its last dimension")
+    _want(bias is None or (bias.dtype == torch.float32
+                           and bias.shape == sw.shape),
+          "bias must be float32 of sw's shape")
+    _want(activation in _ACTS, "activation must be none, relu or tanh")
+    _want(out_dtype in _ELEMS, "out_dtype must be float32, bfloat16 or float16")
+    _want(out is None or (out.dtype == out_dtype and out.is_contiguous()
+                          and out.shape == (*x.shape[:-1], wq.shape[-2])),
+          "out must be contiguous, of out_dtype and of the result's shape")
+
 
 class TorchOps:
     name = "torch_ref"
@@ -64,3 +95,85 @@ class TorchOps:
             if want_sq:
                 acc_sq += (eps * eps * w).sum(dim=0)
         return (acc, acc_sq) if want_sq else acc
+
+    # --- 8-bit rows and products (see ops/hip.py for the definitions) ------
+    def quantize_rows(self, x, out=None):
+        _want(x.dtype in _ELEMS, "x must be float32, bfloat16 or float16")
+        _want(x.dim() >= 1, "x must have at least one dimension")
+        _want(x.shape[-1] <= _MAX_COLS, f"rows of at most {_MAX_COLS} values")
+        if out is not None:
+            _want(out[0].dtype == torch.int8 and out[0].shape == x.shape,
+                  "out[0] must be int8 of x's shape")
+            _want(out[1].dtype == torch.float32
+                  and out[1].shape == x.shape[:-1],
+                  "out[1] must be float32 of x's shape without its last "
+                  "dimension")
+        v = x.detach().to(torch.float64)
+        top = (v.abs().amax(dim=-1) if x.shape[-1]
+               else v.new_zeros(x.shape[:-1]))
+        scale = (top / 127).to(torch.float32).clamp_min(2.0 ** -126)
+        bad = ~torch.isfinite(top)
+        scale = torch.where(bad, torch.full_like(scale, float("nan")), scale)
+        codes = (v / scale.to(torch.float64).unsqueeze(-1)).round()
+        codes = codes.masked_fill(bad.unsqueeze(-1), 0).to(torch.int8)
+        if out is None:
+            return codes, scale
+        out[0].copy_(codes)
+        out[1].copy_(scale)
+        return out
+
+    def int8_matmul(self, xq, sx, wq, sw, bias=None, activation="none",
+                    out_dtype=torch.float32, out=None):
+        _want(xq.dtype == torch.int8, "xq must be int8")
+        _want(xq.dim() >= 1, "xq must have at least one dimension")
+        _want(sx.dtype == torch.float32 and sx.shape == xq.shape[:-1],
+              "sx must be float32 of xq's shape without its last dimension")
+        _want_product(xq, wq, sw, bias, activation, out_dtype, out)
+        if xq.dim() == 1:                    # one row, no axis of rows
+            y = self.int8_matmul(xq[None], sx[None], wq, sw, bias, activation,
+                                 out_dtype)[0]
+            return y if out is None else out.copy_(y)
+        # whole numbers below 2^53: the sums are exact in any order
+        y = xq.to(torch.float64) @ wq.to(torch.float64).transpose(-1, -2)
+        y = y.to(torch.float32) * sx.unsqueeze(-1) * sw.unsqueeze(-2)
+        if bias is not None:
+            y = y + bias.unsqueeze(-2)
+        if activation == "relu":
+            y = y.clamp_min(0)
+        elif activation == "tanh":
+            y = y.tanh()
+        return y.to(out_dtype) if out is None else out.copy_(y)
+
+    def int8_linear(self, x, wq, sw, bias=None, activation="none",
+                    out_dtype=torch.float32, out=None):
+        return self.int8_matmul(*self.quantize_rows(x), wq, sw, bias,
+                                activation, out_dtype, out)
+
+    # --- gradient norm ----------------------------------------------------
+    def global_norm(self, tensors):
+        return self._norm64(tensors).to(torch.float32)
+
+    @staticmethod
+    def _norm64(tensors):
+        _want(len(tensors) > 0, "no tensors")
+        for t in tensors:
+            _want(t.dtype in _ELEMS,
+                  "tensors must be float32, bfloat16 or float16")
+        return torch.stack([t.to(torch.float64).square().sum()
+                            for t in tensors]).sum().sqrt()
+
+    def clip_by_global_norm(self, tensors, max_norm, out=None):
+        norm = self._norm64(tensors)
+        _want(max_norm >= 0, "max_norm must be at least 0")
+        _want(out is None or len(out) == len(tensors),
+              "out must hold as many tensors")
+        c = torch.where(norm > max_norm, max_norm / norm,
+                        torch.ones_like(norm))
+        clipped = [(t.to(torch.float64) * c).to(t.dtype) for t in tensors]
+        if out is not None:
+            for o, t in zip(out, clipped):
+                _want(o.dtype == t.dtype and o.shape == t.shape,
+                      "out must be of its tensor's type and shape")
+                o.copy_(t)
+            clipped = list(out)
+        return clipped, norm.to(torch.float32)
