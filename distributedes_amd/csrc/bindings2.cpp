@@ -18,21 +18,9 @@
 #include <vector>
 
 #include "grad_clip.h"
+#include "int8.h"
 
 extern "C" {
-struct DesInt8Product {  // as in int8.h, which needs a HIP compiler
-  const int8_t* x;
-  const float* sx;
-  const int8_t* w;
-  const float* sw;
-  const float* bias;
-  void* y;
-  int64_t B;
-  int32_t M, N, K;
-  int64_t xsb, xsr, wsb, wsr;
-  int32_t act;
-  int32_t out;
-};
 void des_launch_quantize_rows(const void*, int, int64_t, int64_t, int8_t*,
                               int64_t, int64_t, float*, int64_t, int64_t, int,
                               hipStream_t);
@@ -286,35 +274,61 @@ std::vector<int64_t> check_product(const Tensor& x, const Tensor& wq,
   return shape;
 }
 
-Tensor product(const Tensor& xq_, const Tensor& sx_, const Tensor& wq_,
+// whether every row's last 16 codes lie inside the tensor's storage
+bool whole_rows(const Tensor& t) {
+  int64_t last = t.storage_offset();
+  for (int64_t d = 0; d + 1 < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+  return last + (t.size(-1) + 15) / 16 * 16 <= (int64_t)t.storage().nbytes();
+}
+
+// x: codes with their scales sx, or (sx undefined) float rows
+Tensor product(const Tensor& x_, const Tensor& sx_, const Tensor& wq_,
                const Tensor& sw_, const optional<Tensor>& bias_, int act,
                at::ScalarType out_dtype, const optional<Tensor>& out,
                const std::vector<int64_t>& shape) {
-  Tensor y = out.has_value()
-                 ? *out
-                 : at::empty(shape, sx_.options().dtype(out_dtype));
+  Tensor y =
+      out.has_value() ? *out : at::empty(shape, sw_.options().dtype(out_dtype));
   if (y.numel() == 0) return y;
-  DesInt8Product p;
+  DesInt8Product p = {};
   const bool members = wq_.dim() == 3;
-  Tensor xq = row_view(xq_);
+  Tensor x = row_view(x_);
   if (!members) {
     Rows r;
-    as_rows(xq, &r);
-    if (r.lead != 1) xq = xq.contiguous();
-    as_rows(xq, &r);
+    as_rows(x, &r);
+    if (r.lead != 1) x = x.contiguous();
+    as_rows(x, &r);
     TORCH_CHECK_VALUE(r.rows <= MAX_INT, "too many rows: ", r.rows);
     p.B = 1;
     p.M = (int32_t)r.rows;
     p.xsb = 0;
     p.xsr = r.sr;
   } else {
-    TORCH_CHECK_VALUE(xq.size(1) <= MAX_INT, "too many rows: ", xq.size(1));
-    p.B = xq.size(0);
-    p.M = (int32_t)xq.size(1);
-    p.xsb = xq.stride(0);
-    p.xsr = xq.stride(1);
+    TORCH_CHECK_VALUE(x.size(1) <= MAX_INT, "too many rows: ", x.size(1));
+    p.B = x.size(0);
+    p.M = (int32_t)x.size(1);
+    p.xsb = x.stride(0);
+    p.xsr = x.stride(1);
   }
-  const int64_t K = xq.size(-1);
+  const int64_t K = x.size(-1);
+  Tensor sx;
+  if (sx_.defined()) {
+    sx = sx_.contiguous();
+  } else if (!des_int8_fused(p.M, K)) {
+    const Tensor q = new_codes(x);
+    sx = at::empty(lead_shape(x), x.options().dtype(at::kFloat));
+    launch_quantize(x, q, sx);
+    x = q;
+    p.xsr = members ? q.stride(1) : (K + 15) / 16 * 16;
+    p.xsb = members ? q.stride(0) : 0;
+  }
+  if (sx.defined()) {
+    p.x = x.data_ptr<int8_t>();
+    p.sx = sx.data_ptr<float>();
+    p.xwhole = whole_rows(x);
+  } else {
+    p.xf = x.data_ptr();
+    p.xelem = elem_of(x.scalar_type(), "x");
+  }
   const Tensor wq =
       K > 1 && wq_.stride(-1) != 1 ? wq_.contiguous() : wq_;
   TORCH_CHECK_VALUE(wq.size(-2) <= MAX_INT, "too many channels");
@@ -322,10 +336,9 @@ Tensor product(const Tensor& xq_, const Tensor& sx_, const Tensor& wq_,
   p.K = (int32_t)K;
   p.wsb = members ? wq.stride(0) : 0;
   p.wsr = wq.stride(-2);
-  const Tensor sx = sx_.contiguous(), sw = sw_.contiguous();
+  p.wwhole = whole_rows(wq);
+  const Tensor sw = sw_.contiguous();
   const Tensor bias = bias_.has_value() ? bias_->contiguous() : Tensor();
-  p.x = xq.data_ptr<int8_t>();
-  p.sx = sx.data_ptr<float>();
   p.w = wq.data_ptr<int8_t>();
   p.sw = sw.data_ptr<float>();
   p.bias = bias.defined() ? bias.data_ptr<float>() : nullptr;
@@ -370,11 +383,7 @@ Tensor int8_linear(const Tensor& x_, const Tensor& wq, const Tensor& sw,
   const auto shape = check_product(x_, wq, sw, bias, out_dtype, out);
   check_gpu(x_);
   const c10::DeviceGuard guard(x_.device());
-  const Tensor x = row_view(x_);
-  Tensor q = new_codes(x);
-  Tensor s = at::empty(lead_shape(x), x.options().dtype(at::kFloat));
-  launch_quantize(x, q, s);
-  return product(q, s, wq, sw, bias, act, out_dtype, out, shape);
+  return product(x_, Tensor(), wq, sw, bias, act, out_dtype, out, shape);
 }
 
 // ---------------------------------------------------------------------------

@@ -9,8 +9,10 @@
 // normal number, so that nothing divides by zero.  A row that holds a NaN or an
 // infinity gets scale NaN and codes 0: it shows in every product.
 #pragma once
-#include <hip/hip_runtime.h>
 #include <stdint.h>
+
+#ifdef __HIPCC__
+#include <hip/hip_runtime.h>
 
 namespace des {
 
@@ -76,12 +78,14 @@ __device__ __forceinline__ int row_code(float v, RowScale r) {
 }
 
 }  // namespace des
+#endif  // __HIPCC__
 
 // One batch of products, as the bindings pass it.  Strides in elements; the
 // elements of a row are next to each other.
 struct DesInt8Product {
-  const int8_t* x;      // [B, M, K]
+  const int8_t* x;      // [B, M, K]; null: xf is quantised on the way
   const float* sx;      // [B, M]
+  const void* xf;       // [B, M, K] float rows of type xelem
   const int8_t* w;      // [B, N, K]
   const float* sw;      // [B, N]
   const float* bias;    // nullable [B, N]
@@ -91,4 +95,15 @@ struct DesInt8Product {
   int64_t xsb, xsr, wsb, wsr;
   int32_t act;          // 0 none, 1 relu, 2 tanh
   int32_t out;          // des::Elem
+  int32_t xelem;        // des::Elem
+  // whether a row's last 16 codes may be read whole: the bytes behind the row
+  // belong to its storage
+  int32_t xwhole, wwhole;
 };
+
+// whether int8_linear is one launch (its float rows are quantised inside the
+// product) or two
+inline bool des_int8_fused(int64_t M, int64_t K) {
+  // a block holds its rows' codes in its 64 KB of shared memory
+  return M <= 16 && M * ((K + 63) / 64 * 64 + 16) <= 48 * 1024;
+}
