@@ -5,7 +5,8 @@
 // K = 2^31 / 127^2 = 133144 (the bindings allow 131072), whatever the order, so
 // any split of K gives the same bits.
 //
-// The matrix instruction is v_mfma_i32_16x16x64_i8: a lane gives 16 neighbouring
+// Up to 4 tokens the product is a stream of weights: gemv_kernel.  Otherwise the
+// matrix instruction is v_mfma_i32_16x16x64_i8: a lane gives 16 neighbouring
 // codes of row (lane & 15) at k = 16 * (lane >> 4), and holds the results of
 // column (lane & 15) for rows 4 * (lane >> 4) .. + 3.  Weights are the first
 // operand, so that a lane's four results are four neighbouring channels of one
@@ -20,6 +21,7 @@ using namespace des;
 
 typedef __attribute__((ext_vector_type(4))) int v4i;
 typedef __attribute__((ext_vector_type(4))) float v4f;
+typedef v4i v4i_any __attribute__((aligned(1)));  // at any address
 
 template <typename T, int V>
 struct __attribute__((packed, aligned(sizeof(T)))) Vec { T v[V]; };
@@ -77,6 +79,13 @@ __device__ __forceinline__ void put4(void* y, int64_t at, v4f v, int have,
   }
 }
 
+__device__ __forceinline__ void put1(const DesInt8Product& p, int64_t at,
+                                     float v) {
+  if (p.out == ELEM_F32) reinterpret_cast<float*>(p.y)[at] = v;
+  else if (p.out == ELEM_BF16) reinterpret_cast<Bf16*>(p.y)[at] = from_f32<Bf16>(v);
+  else reinterpret_cast<_Float16*>(p.y)[at] = from_f32<_Float16>(v);
+}
+
 // results of channels n .. n + 3 for token m of member b
 __device__ __forceinline__ void finish4(const DesInt8Product& p, int64_t b,
                                         int m, int n, v4i sum, float sx) {
@@ -95,26 +104,44 @@ __device__ __forceinline__ void finish4(const DesInt8Product& p, int64_t b,
   else put4<_Float16>(p.y, at, v, have, vec);
 }
 
+template <typename T>
+__device__ __forceinline__ void load_floats(const T* src, int k, int K,
+                                            float (&v)[4]) {
+  if (k + 4 <= K) {
+    const auto t = *reinterpret_cast<const Vec<T, 4>*>(src + k);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = to_f32(t.v[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = k + j < K ? to_f32(src[k + j]) : 0.f;
+  }
+}
+
 // Quantises `rows` rows of K floats into shared memory, a row every `step`
-// bytes with zeros up to `kpad`; a thread's slice of every row is the same, so
-// one barrier joins all rows' maxima.
+// bytes with zeros up to `kpad` (a multiple of 4).  A thread's slice of every
+// row is the same, so one barrier joins all rows' maxima; the slice's first
+// four values of the first row are kept in between.
 template <typename T>
 __device__ void quantize_block(const T* x, int64_t xsr, int rows, int K,
                                int kpad, int step, int8_t* codes,
                                float* scales, uint32_t* tops, int waves) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int stride = blockDim.x * 4;
+  float kept[4];
+  load_floats(x, tid * 4, K, kept);
   for (int r = 0; r < rows; ++r) {
     const T* src = x + r * xsr;
     uint32_t top = 0;
     for (int k = tid * 4; k < K; k += stride) {
-      if (k + 4 <= K) {
-        const auto v = *reinterpret_cast<const Vec<T, 4>*>(src + k);
+      float v[4];
+      if (r == 0 && k == tid * 4) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) top = max(top, abs_bits(to_f32(v.v[j])));
+        for (int j = 0; j < 4; ++j) v[j] = kept[j];
       } else {
-        for (int j = k; j < K; ++j) top = max(top, abs_bits(to_f32(src[j])));
+        load_floats(src, k, K, v);
       }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = max(top, abs_bits(v[j]));
     }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1)
@@ -129,20 +156,217 @@ __device__ void quantize_block(const T* x, int64_t xsr, int rows, int K,
     const RowScale rs = row_scale(top);
     if (tid == 0) scales[r] = rs.scale;
     for (int k = tid * 4; k < kpad; k += stride) {
-      union { int word; int8_t b[4]; } o;
-      if (k + 4 <= K) {
-        const auto v = *reinterpret_cast<const Vec<T, 4>*>(src + k);
+      float v[4];
+      if (r == 0 && k == tid * 4) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o.b[j] = (int8_t)row_code(to_f32(v.v[j]), rs);
+        for (int j = 0; j < 4; ++j) v[j] = kept[j];
       } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          o.b[j] = k + j < K ? (int8_t)row_code(to_f32(src[k + j]), rs) : 0;
+        load_floats(src, k, K, v);
       }
+      union { int word; int8_t b[4]; } o;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o.b[j] = (int8_t)row_code(v[j], rs);
       *reinterpret_cast<int*>(codes + r * step + k) = o.word;
     }
   }
   __syncthreads();
+}
+
+// Copies rows of K codes into shared memory, a row every `step` bytes with
+// zeros up to `kpad` (a multiple of 16).
+__device__ void stage_block(const int8_t* x, int64_t xsr, int rows, int K,
+                            int kpad, int step, int8_t* codes, bool whole) {
+  for (int r = 0; r < rows; ++r)
+    for (int k = threadIdx.x * 16; k < kpad; k += blockDim.x * 16)
+      *reinterpret_cast<v4i*>(codes + r * step + k) =
+          load_tail(x + r * xsr + k, K - k, whole);
+  __syncthreads();
+}
+
+// One token to MR: memory bound, every weight is read once for 2 MR operations.
+// A row of weights goes to L neighbouring lanes (1 to 64, a power of 2), so a
+// wave's load is 64 / L pieces of 16 L bytes; U such loads are under way, and
+// the next U begin before their products.  Products are v_dot4_i32_i8 with the
+// token's codes from shared memory; L lanes' sums are joined at the row's end.
+//
+// The matrix instruction would want 16 rows in pieces of 64 bytes: for a layer
+// of 256 x 376 for each of 10000 members that reads 4.2 TB/s, this 6.1 (a plain
+// read of as much: 7.0), and rows of 3136 codes 5.1 against 6.3.
+template <typename X, int MR, int U, bool ONCE>
+__global__ __launch_bounds__(256) void gemv_kernel(DesInt8Product p, int lbits,
+                                                   int rows_a_wave) {
+  extern __shared__ __align__(16) int8_t shared[];
+  constexpr bool FLOATS = sizeof(X) != 1;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int waves = blockDim.x >> 6;
+  const int nblocks = (p.N + waves * rows_a_wave - 1) / (waves * rows_a_wave);
+  const int64_t b = blockIdx.x / nblocks;
+  const int nb = (int)(blockIdx.x - b * nblocks);
+  const int kpad = (p.K + 15) / 16 * 16, step = kpad + 16;
+  float* scales = reinterpret_cast<float*>(shared);
+  int8_t* codes = shared + 16;
+  int* sums = reinterpret_cast<int*>(codes + p.M * step);
+  const int L = 1 << lbits, per = 64 >> lbits;  // lanes a row, rows a load
+  const int li = lane & (L - 1), sub = lane >> lbits;
+  const int kend = p.wwhole ? kpad : p.K / 16 * 16;
+  const int8_t* wb = p.w + b * p.wsb;
+  const int first = (nb * waves + wave) * rows_a_wave;
+  const int last = min(first + rows_a_wave, p.N);
+
+  v4i next[U];  // the next turn's weights: loads run ahead by one
+  const int8_t* wr[U];
+  auto rows_at = [&](int n0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      wr[u] = wb + (int64_t)min(n0 + u * per + sub, p.N - 1) * p.wsr;
+  };
+  auto fetch = [&](int k) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const v4i_any* at = reinterpret_cast<const v4i_any*>(wr[u] + k);
+      next[u] = k >= kend ? v4i{0, 0, 0, 0}
+                : ONCE    ? __builtin_nontemporal_load(at)
+                          : *at;
+    }
+  };
+  rows_at(first);
+  if (first < last) fetch(li * 16);  // under way while the token is quantised
+  const int ch = first + lane;       // a wave has at most 64 channels
+  float sw = 0.f, bias = 0.f;
+  if (ch < last) {
+    sw = p.sw[b * p.N + ch];
+    if (p.bias) bias = p.bias[b * p.N + ch];
+  }
+
+  if constexpr (FLOATS) {
+    uint32_t* tops = reinterpret_cast<uint32_t*>(sums + waves * 64 * MR);
+    quantize_block((const X*)p.xf + b * p.xsb, p.xsr, p.M, p.K, kpad, step,
+                   codes, scales, tops, waves);
+  } else {
+    stage_block(p.x + b * p.xsb, p.xsr, p.M, p.K, kpad, step, codes, p.xwhole);
+  }
+
+  int* mine = sums + wave * 64 * MR;
+  for (int n0 = first; n0 < last; n0 += U * per) {
+    if (kend == 0) rows_at(n0);  // no whole piece: the loop below has no turn
+    int acc[U][MR];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int m = 0; m < MR; ++m) acc[u][m] = 0;
+    auto add = [&](int k, const v4i (&w)[U]) {
+#pragma unroll
+      for (int m = 0; m < MR; ++m) {
+        if (m > 0 && m >= p.M) break;
+        const v4i x = *reinterpret_cast<const v4i*>(codes + m * step + k);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            acc[u][m] = __builtin_amdgcn_sdot4(w[u][j], x[j], acc[u][m], false);
+      }
+    };
+    v4i tail[U];
+    const bool odd = kend < p.K && li == 0;
+    if (odd) {  // a row's last codes, none behind them read
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        tail[u] = load_tail(wr[u] + kend, p.K - kend, false);
+    }
+    for (int k = li * 16; k - li * 16 < kend; k += L * 16) {
+      v4i w[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) w[u] = next[u];
+      if (k - li * 16 + L * 16 < kend) {
+        fetch(k + L * 16);
+      } else if (n0 + U * per < last) {
+        rows_at(n0 + U * per);
+        fetch(li * 16);
+      }
+      add(min(k, kpad), w);  // w = 0 behind the row
+    }
+    if (odd) add(kend, tail);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int m = 0; m < MR; ++m) {
+        for (int off = L >> 1; off > 0; off >>= 1)
+          acc[u][m] += __shfl_xor(acc[u][m], off);
+        const int at = n0 - first + u * per + sub;
+        if (li == 0 && at < 64) mine[m * 64 + at] = acc[u][m];
+      }
+  }
+  __syncthreads();
+  // one lane a channel: the factors were fetched at the start, and the
+  // activation runs on whole waves
+  if (ch < last) {
+#pragma unroll
+    for (int m = 0; m < MR; ++m) {
+      if (m >= p.M) break;
+      const float sx = FLOATS ? scales[m] : p.sx[b * p.M + m];
+      put1(p, (b * p.M + m) * p.N + ch,
+           finish(mine[m * 64 + lane], sx, sw, bias, p.act));
+    }
+  }
+}
+
+template <typename X, int MR, int U, bool ONCE>
+void launch_gemv(const DesInt8Product& p, int lbits, int rows_a_wave,
+                 hipStream_t stream) {
+  const int64_t parts = (p.N + (int64_t)rows_a_wave - 1) / rows_a_wave;
+  const int waves = (int)std::min<int64_t>(4, parts);
+  const int64_t nblocks = (parts + waves - 1) / waves;
+  const size_t bytes = 16 + p.M * ((p.K + 15) / 16 * 16 + 16) +
+                       waves * 64 * MR * 4 + p.M * waves * 4;
+  hipLaunchKernelGGL((gemv_kernel<X, MR, U, ONCE>),
+                     dim3((uint32_t)(p.B * nblocks)), dim3(64 * waves), bytes,
+                     stream, p, lbits, rows_a_wave);
+}
+
+// How many lanes take a row, how many rows a wave takes, and whether its loads
+// pass the caches by.  Measured over 0.5 to 1 GB of weights, M = 1:
+//  - up to 32 MB: latency counts.  A row to as many lanes as it fills, one load
+//    a row and turn, and as many waves as that gives.
+//  - weights that no cache would keep (256 MB), rows that begin on lines of
+//    128 bytes: past the caches, a line a turn and row.  K = 376 (rows of 384):
+//    4 lanes 292 us, 8 163, 16 167, 32 192; through the caches 180.
+//  - such weights in long rows that do not: 64 lanes, so that few lines are
+//    fetched in halves.  K = 3136: 509 us, 16 lanes 576.
+//  - all others: through the caches, which join halves of lines, and few lanes,
+//    which have fewer sums to join.  K = 200 (208): 2 lanes 255 us, 4 130, 8 104,
+//    16 99; past the caches 150.  K = 48: 1 lane 139, 2 124, 4 138.
+template <typename X, int MR>
+void choose_gemv_rows(const DesInt8Product& p, hipStream_t stream) {
+  const int64_t bytes = p.B * (int64_t)p.N * p.K;
+  auto lanes = [&](int codes, int least, int most) {  // as bits
+    int bits = least;
+    while (bits < most && (int64_t)codes << bits < p.K) ++bits;
+    return bits;
+  };
+  if (bytes <= 32 << 20) {
+    const int bits = lanes(16, 0, 6);
+    launch_gemv<X, MR, 1, false>(p, bits, 64 >> bits, stream);
+    return;
+  }
+  const int rows = p.K >= 1024 ? 16 : 64;
+  const bool lines =
+      ((uintptr_t)p.w | (uintptr_t)p.wsr | (uintptr_t)p.wsb) % 128 == 0;
+  const bool once = bytes >= 256 << 20;
+  if (once && lines && p.K > 96)
+    launch_gemv<X, MR, 2, true>(p, 3, rows, stream);
+  else if (once && p.K >= 2048)
+    launch_gemv<X, MR, 4, true>(p, 6, rows, stream);
+  else
+    launch_gemv<X, MR, 2, false>(p, p.K <= 16 ? 0 : lanes(32, 1, 4), rows,
+                                 stream);
+}
+
+template <typename X>
+void choose_gemv(const DesInt8Product& p, hipStream_t stream) {
+  if (p.M == 1)
+    choose_gemv_rows<X, 1>(p, stream);
+  else
+    choose_gemv_rows<X, 4>(p, stream);
 }
 
 // Few rows: weights go straight from memory into the matrix instruction's
@@ -303,16 +527,21 @@ void choose_stream(const DesInt8Product& p, hipStream_t stream) {
 
 extern "C" void des_launch_int8_product(const DesInt8Product* p,
                                         hipStream_t stream) {
-  if (p->x) {
-    if (p->M > 64 && p->N > 32)
-      launch_stream<int8_t, 4, 4>(*p, 1, 1, stream);
+  const DesInt8Product& q = *p;
+  const bool gemv = q.M <= 4 && q.M * (int64_t)q.K <= 48 * 1024;
+  if (q.x) {
+    if (gemv)
+      choose_gemv<int8_t>(q, stream);
+    else if (q.M > 64 && q.N > 32)
+      launch_stream<int8_t, 4, 4>(q, 1, 1, stream);
     else
-      choose_stream<int8_t>(*p, stream);
-  } else if (p->xelem == ELEM_F32) {
-    choose_stream<float>(*p, stream);
-  } else if (p->xelem == ELEM_BF16) {
-    choose_stream<Bf16>(*p, stream);
+      choose_stream<int8_t>(q, stream);
+  } else if (q.xelem == ELEM_F32) {
+    gemv ? choose_gemv<float>(q, stream) : choose_stream<float>(q, stream);
+  } else if (q.xelem == ELEM_BF16) {
+    gemv ? choose_gemv<Bf16>(q, stream) : choose_stream<Bf16>(q, stream);
   } else {
-    choose_stream<_Float16>(*p, stream);
+    gemv ? choose_gemv<_Float16>(q, stream)
+         : choose_stream<_Float16>(q, stream);
   }
 }
