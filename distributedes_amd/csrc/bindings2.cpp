@@ -25,6 +25,8 @@ void des_launch_quantize_rows(const void*, int, int64_t, int64_t, int8_t*,
                               int64_t, int64_t, float*, int64_t, int64_t, int,
                               hipStream_t);
 void des_launch_int8_product(const DesInt8Product*, hipStream_t);
+void des_launch_pack_rows(const int8_t*, int64_t, int64_t, int8_t*, int64_t,
+                          int64_t, int, hipStream_t);
 void des_launch_square_sums(const DesClipTable*, int64_t, double*,
                             hipStream_t);
 void des_launch_norm(const double*, int, float*, hipStream_t);
@@ -281,6 +283,26 @@ bool whole_rows(const Tensor& t) {
   return last + (t.size(-1) + 15) / 16 * 16 <= (int64_t)t.storage().nbytes();
 }
 
+// The tiled kernel reads whole pieces of 16 codes at addresses of 16: rows that
+// lie otherwise are copied.  `kept` holds the copy until the product is
+// launched.
+const int8_t* aligned_rows(const int8_t* rows, int64_t* sb, int64_t* sr,
+                           int64_t B, int64_t n, int64_t K, bool whole,
+                           const Tensor& like, Tensor* kept) {
+  const int64_t lead = B > 1 && *sb != 0 ? B : 1;
+  if (whole && reinterpret_cast<uintptr_t>(rows) % 16 == 0 &&
+      (n == 1 || *sr % 16 == 0) && (lead == 1 || *sb % 16 == 0))
+    return rows;
+  const int64_t step = (K + 15) / 16 * 16;
+  *kept = at::empty({lead * n * step}, like.options().dtype(at::kChar));
+  des_launch_pack_rows(rows, *sb, *sr, kept->data_ptr<int8_t>(), lead, n,
+                       (int)K, cur_stream());
+  CHECK_LAUNCH();
+  *sr = step;
+  *sb = lead == 1 ? 0 : n * step;
+  return kept->data_ptr<int8_t>();
+}
+
 // x: codes with their scales sx, or (sx undefined) float rows
 Tensor product(const Tensor& x_, const Tensor& sx_, const Tensor& wq_,
                const Tensor& sw_, const optional<Tensor>& bias_, int act,
@@ -348,6 +370,11 @@ Tensor product(const Tensor& x_, const Tensor& sx_, const Tensor& wq_,
   const double tiles = (double)p.B * ((p.M + 15) / 16) * ((p.N + 15) / 16);
   TORCH_CHECK_VALUE(tiles <= (double)MAX_INT, "a product of ", p.B, " x ", p.M,
                     " x ", p.N, " results is too large for one call");
+  Tensor x_copy, w_copy;
+  if (K > 0 && des_int8_plan(p.B, p.M, p.N, p.K) == DES_INT8_TILED) {
+    p.x = aligned_rows(p.x, &p.xsb, &p.xsr, p.B, p.M, K, p.xwhole, y, &x_copy);
+    p.w = aligned_rows(p.w, &p.wsb, &p.wsr, p.B, p.N, K, p.wwhole, y, &w_copy);
+  }
   des_launch_int8_product(&p, cur_stream());
   CHECK_LAUNCH();
   return y;

@@ -12,6 +12,7 @@
 // operand, so that a lane's four results are four neighbouring channels of one
 // token: one store.
 #include <algorithm>
+#include <type_traits>
 
 #include "int8.h"
 
@@ -398,9 +399,10 @@ __global__ __launch_bounds__(1024) void stream_kernel(DesInt8Product p, int wn,
 
   if constexpr (FLOATS) {
     const int rows = min(16, p.M - m0);
+    const X* xf = (const X*)p.xf + b * p.xsb + m0 * p.xsr;
     uint32_t* tops = reinterpret_cast<uint32_t*>(codes + rows * xstep);
-    quantize_block((const X*)p.xf + b * p.xsb + m0 * p.xsr, p.xsr, rows, p.K,
-                   steps * 64, xstep, codes, scales, tops, waves);
+    quantize_block(xf, p.xsr, rows, p.K, steps * 64, xstep, codes, scales, tops,
+                   waves);
   }
   const int8_t* wr[NT];
   const int8_t* xr[MT];
@@ -506,42 +508,363 @@ void launch_stream(const DesInt8Product& p, int wn, int wk,
                      dim3(64 * waves), bytes, stream, p, wn, wk);
 }
 
-// Few rows.  Many members (or channels) fill the chip with waves of 64
-// channels; else a wave has 16 and K is split until about 2048 waves run.
+// Many members fill the chip with waves of 64 channels (or, for 17 to 32
+// tokens, 32 channels); else a wave has 16 channels, and 8 to 16 of them share
+// K.  For one policy of 512 x 3136: 16 to 128 tokens 5.2 us, in groups of 16
+// tokens; 256 tokens in groups of 32 6.8; 512 tokens in groups of 32 x 32 8.7.
 template <typename X>
 void choose_stream(const DesInt8Product& p, hipStream_t stream) {
   const int64_t groups = (p.N + 15) / 16, steps = (p.K + 63) / 64;
-  const int64_t mb = (p.M + 15) / 16;
-  if (p.B * mb * groups >= 4 * 2048 && groups >= 4) {
+  const int64_t blocks = p.B * ((p.M + 15) / 16) * groups;
+  if (p.M <= 16 && blocks >= 4 * 2048 && groups >= 4) {
     launch_stream<X, 1, 4>(p, (int)std::min<int64_t>(4, (groups + 3) / 4), 1,
                            stream);
     return;
   }
+  if constexpr (sizeof(X) == 1) {
+    if (p.M > 16 && p.B > 1 && blocks >= 4096) {
+      launch_stream<X, 2, 2>(p, (int)std::min<int64_t>(4, (groups + 1) / 2), 1,
+                             stream);
+      return;
+    }
+    if (blocks > 1024) {
+      launch_stream<X, 2, 2>(p, 1, steps >= 4 ? 4 : 1, stream);
+      return;
+    }
+    if (blocks > 256 && p.M > 16) {
+      launch_stream<X, 2, 1>(p, 1, steps >= 8 ? 8 : steps >= 4 ? 4 : 1, stream);
+      return;
+    }
+  }
   int wn = 1, wk = 1;
-  while (wk < 16 && p.B * mb * groups * wk < 2048 && steps >= 4 * wk) wk *= 2;
+  while (wk < 8 && blocks * wk < 2048 && steps >= 2 * wk) wk *= 2;
+  if (wk == 8 && blocks <= 64 && steps >= 32) wk = 16;
   while (wn * wk < 4 && wn < groups) wn *= 2;
   launch_stream<X, 1, 1>(p, wn, wk, stream);
 }
 
+typedef __attribute__((ext_vector_type(16))) int v16i;
+
+// memory -> shared memory without registers in between: lane l's 16 bytes go
+// to `to` + 16 l
+__device__ __forceinline__ void load_shared(const int8_t* from, int8_t* to) {
+  __builtin_amdgcn_global_load_lds(
+      (const __attribute__((address_space(1))) void*)from,
+      (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+
+// until at most N loads are under way
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) |
+                             ((N >> 4) << 14));
+}
+
+// Writes Q x 4 results: of tokens m[q], channels n .. n + 3 (`have` of them
+// within the row).
+template <int Q>
+__device__ __forceinline__ void put_rows(const DesInt8Product& p, int64_t b,
+                                         const int (&m)[Q], int n, int have,
+                                         const v4f (&v)[Q]) {
+#pragma unroll
+  for (int q = 0; q < Q; ++q) {
+    if (m[q] >= p.M || have <= 0) continue;
+    const int64_t at = (b * p.M + m[q]) * p.N + n;
+    if (have >= 4) {
+      if (p.out == ELEM_F32) {
+        Vec<float, 4> o = {{v[q][0], v[q][1], v[q][2], v[q][3]}};
+        reinterpret_cast<Vec<float, 4>*>(reinterpret_cast<float*>(p.y) + at)[0] = o;
+      } else {
+        Vec<uint16_t, 4> o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          o.v[e] = p.out == ELEM_BF16
+                       ? from_f32<Bf16>(v[q][e]).bits
+                       : __builtin_bit_cast(uint16_t, (_Float16)v[q][e]);
+        reinterpret_cast<Vec<uint16_t, 4>*>(reinterpret_cast<uint16_t*>(p.y) +
+                                            at)[0] = o;
+      }
+    } else {
+      put1(p, at, v[q][0]);
+      if (have > 1) put1(p, at + 1, v[q][1]);
+      if (have > 2) put1(p, at + 2, v[q][2]);
+    }
+  }
+}
+
+// Many rows: a block has WN x WM waves, each with NT x MT blocks of 32 x 32
+// results (channels x tokens), and takes K in stages of BK codes through
+// shared memory, S stages in a ring: while one is multiplied, S - 1 are on
+// their way.  A stage's rows lie BK bytes apart; the 16-byte piece c of row r
+// is kept at place c ^ (r & 7) (BK = 64: two rows share the banks' 128 bytes,
+// c ^ (r / 2 & 3)), so that the 8 lanes that read together (8 rows, the same
+// piece) meet 8 different places.  Loads write lanes' pieces next to each
+// other, so the places are exchanged where the pieces are read from memory.
+//
+// v_mfma_i32_32x32x32_i8: a lane gives 16 codes of row (lane & 31) at
+// k = 16 * (lane >> 5), and holds the results of token (lane & 31) for channels
+// 8 * (i / 4) + 4 * (lane >> 5) + i % 4, i < 16.
+//
+// The end is kept short: every instruction of a kernel comes from memory once a
+// launch, and 10 KB of unrolled epilogue took 10 us.
+template <int WN, int WM, int NT, int MT, int BK, int S>
+__global__ __launch_bounds__(64 * WN * WM) void tiled_kernel(
+    DesInt8Product p, uint32_t nblocks, uint32_t mblocks) {
+  constexpr int THREADS = 64 * WN * WM;
+  constexpr int BN = 32 * WN * NT, BM = 32 * WM * MT;
+  constexpr int ROW_PIECES = BK / 16;
+  constexpr int PIECES = (BN + BM) * ROW_PIECES / THREADS;  // a thread's
+  constexpr int STAGE = (BN + BM) * BK;
+  extern __shared__ __align__(16) int8_t shared[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wn = wave % WN, wm = wave / WN;
+  uint32_t id = blockIdx.x;
+  const int nb = id % nblocks;
+  id /= nblocks;
+  const int mb = id % mblocks;
+  const int64_t b = id / mblocks;
+  const int n0 = nb * BN, m0 = mb * BM;
+  auto place = [](int r) { return BK == 128 ? r & 7 : r >> 1 & 3; };
+
+  // a thread's pieces of a stage: rows of weights, then rows of tokens
+  const int8_t* src[PIECES];
+  int col[PIECES];
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    const int at = i * THREADS + tid, r = at / ROW_PIECES;
+    col[i] = ((at % ROW_PIECES) ^ place(r)) * 16;
+    src[i] = r < BN ? p.w + b * p.wsb + (int64_t)min(n0 + r, p.N - 1) * p.wsr
+                    : p.x + b * p.xsb +
+                          (int64_t)min(m0 + r - BN, p.M - 1) * p.xsr;
+  }
+  // pieces behind a row's end are read at its begin: their products are masked
+  auto fetch = [&](int k0, int stage) {
+    int8_t* to = shared + stage * STAGE + wave * 1024;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int k = k0 + col[i];
+      load_shared(src[i] + (k < p.K ? k : 0), to + i * THREADS * 16);
+    }
+  };
+
+  const int half = lane >> 5, row = lane & 31;
+  // the factors: a lane's token here, its four channels in the epilogue
+  constexpr int LANES = NT * 8, TOKENS = 64 / LANES;  // of one turn there
+  const int n = n0 + wn * NT * 32 + lane % LANES * 4;
+  const int have = p.N - n;
+  float sx[MT], sw[4], bias[4];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+    sx[i] = p.sx[b * p.M + min(m0 + (wm * MT + i) * 32 + row, p.M - 1)];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int64_t at = b * p.N + min(n + e, p.N - 1);
+    sw[e] = p.sw[at];
+    bias[e] = p.bias ? p.bias[at] : 0.f;
+  }
+  // these have arrived: from here on only stages are counted
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) fetch(s * BK, s);
+
+  v16i acc[NT][MT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[j][i][e] = 0;
+
+  const int wrow = wn * NT * 32 + row, xrow = BN + wm * MT * 32 + row;
+  auto step = [&](const int8_t* stage, int left, auto masked) {
+#pragma unroll
+    for (int s = 0; s < BK / 32; ++s) {
+      v4i a[NT], x[MT];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const int r = wrow + 32 * j;
+        a[j] = *reinterpret_cast<const v4i*>(
+            stage + r * BK + (((2 * s + half) ^ place(r)) << 4));
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const int r = xrow + 32 * i;
+        x[i] = *reinterpret_cast<const v4i*>(
+            stage + r * BK + (((2 * s + half) ^ place(r)) << 4));
+      }
+      if constexpr (decltype(masked)::value) {  // tokens are 0 behind K
+        const int have_k = left - (2 * s + half) * 16;
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int c = have_k - 4 * j;
+            x[i][j] &= c >= 4 ? -1 : c <= 0 ? 0 : (1 << (8 * c)) - 1;
+          }
+      }
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+          acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[j], x[i],
+                                                            acc[j][i], 0, 0, 0);
+    }
+  };
+
+  // A turn waits for its stage's own loads, then at the barrier for all waves':
+  // by then they have also read the stage before it, whose place the next loads
+  // take.  Loads behind the last stage repeat row begins, to keep the count.
+  int turn = 0, k0 = 0;
+  for (; k0 + BK <= p.K; k0 += BK) {
+    wait_loads<PIECES * (S - 2)>();
+    __builtin_amdgcn_s_barrier();
+    fetch(k0 + (S - 1) * BK, turn == 0 ? S - 1 : turn - 1);
+    step(shared + turn * STAGE, BK, std::false_type{});
+    turn = turn == S - 1 ? 0 : turn + 1;
+  }
+  if (k0 < p.K) {
+    wait_loads<PIECES * (S - 2)>();
+    __builtin_amdgcn_s_barrier();
+    step(shared + turn * STAGE, p.K - k0, std::true_type{});
+  }
+  wait_loads<0>();
+  __syncthreads();
+
+  // 32 tokens x 32 NT channels at a time through the wave's own part of shared
+  // memory, to store whole rows
+  constexpr int ROW = NT * 32 + 4;
+  int* mine = reinterpret_cast<int*>(shared) + wave * 32 * ROW;
+#pragma unroll 1
+  for (int i = 0; i < MT; ++i) {
+    float sxi = sx[0];
+#pragma unroll
+    for (int ii = 0; ii < MT; ++ii) {
+      if (i != ii) continue;
+      sxi = sx[ii];
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const v4i sum = {acc[j][ii][4 * g], acc[j][ii][4 * g + 1],
+                           acc[j][ii][4 * g + 2], acc[j][ii][4 * g + 3]};
+          *reinterpret_cast<v4i*>(mine + row * ROW + j * 32 + 8 * g +
+                                  4 * half) = sum;
+        }
+    }
+    __builtin_amdgcn_wave_barrier();
+    auto rows = [&](auto count, int t0) {
+      constexpr int Q = decltype(count)::value;
+      v4f v[Q];
+      int m[Q];
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        const int t = t0 + q * TOKENS + lane / LANES;
+        m[q] = m0 + (wm * MT + i) * 32 + t;
+        const v4i sum = *reinterpret_cast<const v4i*>(mine + t * ROW +
+                                                      lane % LANES * 4);
+        const float s = __shfl(sxi, t);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[q][e] = finish(sum[e], s, sw[e], bias[e], Q == 1 ? p.act : p.act & 1);
+      }
+      put_rows<Q>(p, b, m, n, have, v);
+    };
+    if (p.act == 2) {
+#pragma unroll 1
+      for (int t0 = 0; t0 < 32; t0 += TOKENS)
+        rows(std::integral_constant<int, 1>{}, t0);
+    } else {
+#pragma unroll 1
+      for (int t0 = 0; t0 < 32; t0 += 4 * TOKENS)
+        rows(std::integral_constant<int, 4>{}, t0);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+template <int WN, int WM, int NT, int MT, int BK, int S>
+void launch_tiled(const DesInt8Product& p, hipStream_t stream) {
+  constexpr int BN = 32 * WN * NT, BM = 32 * WM * MT;
+  constexpr int bytes = std::max(S * (BN + BM) * BK,
+                                 WN * WM * 32 * (NT * 32 + 4) * 4);
+  const uint32_t nblocks = (p.N + (int64_t)BN - 1) / BN;
+  const uint32_t mblocks = (p.M + (int64_t)BM - 1) / BM;
+  auto kernel = tiled_kernel<WN, WM, NT, MT, BK, S>;
+  if (bytes > 64 * 1024)
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                              hipFuncAttributeMaxDynamicSharedMemorySize,
+                              bytes);
+  hipLaunchKernelGGL(kernel, dim3((uint32_t)(p.B * nblocks * mblocks)),
+                     dim3(64 * WN * WM), bytes, stream, p, nblocks, mblocks);
+}
+
+// The largest tiles that give each of the chip's 256 units one, measured in us:
+//                        256 x 256  128 x 128  128 x 64  64 x 64
+//   8192 x 4096 x 4096       152        201       186      227
+//   8192 x  512 x 3136        52         25.0      25.8     36
+//   2048 x 2048 x 2048        37         18.7      17.7     20
+//   1024 x  512 x 3136        45         22        15.1     10.7
+void choose_tiled(const DesInt8Product& p, hipStream_t stream) {
+  auto tiles = [&](int64_t n, int64_t m) {
+    return p.B * ((p.N + n - 1) / n) * ((p.M + m - 1) / m);
+  };
+  if (tiles(256, 256) >= 256)
+    launch_tiled<2, 4, 4, 2, 128, 2>(p, stream);
+  else if (tiles(128, 128) >= 256)
+    launch_tiled<2, 2, 2, 2, 64, 3>(p, stream);
+  else if (tiles(128, 64) >= 256)
+    launch_tiled<2, 2, 2, 1, 128, 2>(p, stream);
+  else
+    launch_tiled<2, 2, 1, 1, 128, 3>(p, stream);
+}
+
+// codes -> rows every `step` bytes, with zeros behind them
+__global__ __launch_bounds__(256) void pack_rows_kernel(
+    const int8_t* __restrict__ from, int64_t sb, int64_t sr,
+    int8_t* __restrict__ to, int64_t rows, int K, int step, int64_t pieces) {
+  const int per = step / 16;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < pieces;
+       i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / per, b = r / rows;
+    const int k = (int)(i - r * per) * 16;
+    reinterpret_cast<v4i*>(to)[i] =
+        load_tail(from + b * sb + (r - b * rows) * sr + k, K - k, false);
+  }
+}
+
 }  // namespace
+
+extern "C" void des_launch_pack_rows(const int8_t* from, int64_t sb, int64_t sr,
+                                     int8_t* to, int64_t B, int64_t rows,
+                                     int K, hipStream_t stream) {
+  const int step = (K + 15) / 16 * 16;
+  const int64_t pieces = B * rows * (step / 16);
+  if (pieces == 0) return;
+  hipLaunchKernelGGL(pack_rows_kernel,
+                     dim3((uint32_t)std::min<int64_t>((pieces + 255) / 256,
+                                                      8192)),
+                     dim3(256), 0, stream, from, sb, sr, to, rows, K, step,
+                     pieces);
+}
 
 extern "C" void des_launch_int8_product(const DesInt8Product* p,
                                         hipStream_t stream) {
   const DesInt8Product& q = *p;
-  const bool gemv = q.M <= 4 && q.M * (int64_t)q.K <= 48 * 1024;
-  if (q.x) {
-    if (gemv)
-      choose_gemv<int8_t>(q, stream);
-    else if (q.M > 64 && q.N > 32)
-      launch_stream<int8_t, 4, 4>(q, 1, 1, stream);
-    else
-      choose_stream<int8_t>(q, stream);
+  const DesInt8Plan plan = des_int8_plan(q.B, q.M, q.N, q.K);
+  if (plan == DES_INT8_TILED) {
+    choose_tiled(q, stream);
+  } else if (q.x) {
+    plan == DES_INT8_GEMV ? choose_gemv<int8_t>(q, stream)
+                          : choose_stream<int8_t>(q, stream);
   } else if (q.xelem == ELEM_F32) {
-    gemv ? choose_gemv<float>(q, stream) : choose_stream<float>(q, stream);
+    plan == DES_INT8_GEMV ? choose_gemv<float>(q, stream)
+                          : choose_stream<float>(q, stream);
   } else if (q.xelem == ELEM_BF16) {
-    gemv ? choose_gemv<Bf16>(q, stream) : choose_stream<Bf16>(q, stream);
+    plan == DES_INT8_GEMV ? choose_gemv<Bf16>(q, stream)
+                          : choose_stream<Bf16>(q, stream);
   } else {
-    gemv ? choose_gemv<_Float16>(q, stream)
-         : choose_stream<_Float16>(q, stream);
+    plan == DES_INT8_GEMV ? choose_gemv<_Float16>(q, stream)
+                          : choose_stream<_Float16>(q, stream);
   }
 }
