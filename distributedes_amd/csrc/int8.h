@@ -61,18 +61,40 @@ __device__ __forceinline__ RowScale row_scale(uint32_t top) {
   return r;
 }
 
-// The code of v.  rint(v * inv) is at most one step off, and only next to a
-// border; the remainder v - q s has at most 24 bits there, so the fma is exact
-// and tells on which side of the border (or on it) v lies.
-__device__ __forceinline__ int row_code(float v, RowScale r) {
-  float q = rintf(v * r.inv);
-  float rem = fmaf(-q, r.scale, v);
-  float twice = 2.0f * fabsf(rem);
-  if (twice >= r.scale && r.inv != 0.f) {
-    if (twice > r.scale || ((int)q & 1)) q += rem > 0.f ? 1.0f : -1.0f;
+// Four codes in one word.  Adding 1.5 * 2^23 rounds v * inv to a whole number,
+// ties to even, which the sum's low byte holds as int8.  That is at most one
+// step off, and only next to a border of two codes; the remainder v - q s has at
+// most 24 bits there, so its fma is exact and tells on which side of the border
+// (or on it) v lies.
+__device__ __forceinline__ uint32_t row_codes(const float (&v)[4], RowScale r) {
+  const float whole = 12582912.0f, border = 0.5f * r.scale;
+  float t[4], rem[4];
+  bool near = false;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    t[j] = fmaf(v[j], r.inv, whole);
+    rem[j] = fmaf(whole - t[j], r.scale, v[j]);
+    near |= fabsf(rem[j]) >= border;
   }
-  return r.inv == 0.f ? 0 : (int)q;
+  // scales below 2^-125 have borders that half a scale cannot hold
+  if (__builtin_expect(near || r.scale < 2.3509887e-38f, 0)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float twice = 2.0f * fabsf(rem[j]);
+      if (twice > r.scale ||
+          (twice == r.scale && (__float_as_uint(t[j]) & 1)))
+        t[j] += rem[j] > 0.f ? 1.0f : -1.0f;
+    }
+  }
+  if (!(r.inv > 0.f)) return 0;
+  const uint32_t low = __builtin_amdgcn_perm(
+      __float_as_uint(t[1]), __float_as_uint(t[0]), 0x0c0c0400u);
+  return low | __builtin_amdgcn_perm(__float_as_uint(t[3]),
+                                     __float_as_uint(t[2]), 0x04000c0cu);
 }
+
+template <typename T, int V>
+struct __attribute__((packed, aligned(sizeof(T)))) Vec { T v[V]; };
 
 }  // namespace des
 #endif  // __HIPCC__

@@ -24,9 +24,6 @@ typedef __attribute__((ext_vector_type(4))) int v4i;
 typedef __attribute__((ext_vector_type(4))) float v4f;
 typedef v4i v4i_any __attribute__((aligned(1)));  // at any address
 
-template <typename T, int V>
-struct __attribute__((packed, aligned(sizeof(T)))) Vec { T v[V]; };
-
 // 16 codes from any address
 __device__ __forceinline__ v4i load16(const int8_t* p) {
   v4i v;
@@ -164,10 +161,7 @@ __device__ void quantize_block(const T* x, int64_t xsr, int rows, int K,
       } else {
         load_floats(src, k, K, v);
       }
-      union { int word; int8_t b[4]; } o;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o.b[j] = (int8_t)row_code(v[j], rs);
-      *reinterpret_cast<int*>(codes + r * step + k) = o.word;
+      *reinterpret_cast<uint32_t*>(codes + r * step + k) = row_codes(v, rs);
     }
   }
   __syncthreads();

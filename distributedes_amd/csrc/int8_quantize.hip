@@ -1,42 +1,178 @@
 // quantize_rows: float rows -> 8-bit codes and one fp32 scale a row (int8.h has
-// the definition).  Memory bound: a row is read, its codes written.
+// the definition).
+//
+// Memory bound: a row is read once and held in registers between its maximum
+// and its codes.  About 6 operations a value (see row_codes) are 2 to 4 times
+// less than the loads take.
+#include <algorithm>
+
 #include "int8.h"
 
 namespace {
 
 using namespace des;
 
+struct Rows {
+  const void* x;
+  int8_t* q;
+  float* scale;
+  int64_t xsl, xsr, qsl, qsr;
+  uint32_t lead, rows;
+  int32_t cols;
+};
+
 template <typename T>
-__global__ __launch_bounds__(256) void quantize_rows_kernel(
-    const T* __restrict__ x, int64_t xsl, int64_t xsr, int8_t* __restrict__ q,
-    int64_t qsl, int64_t qsr, float* __restrict__ scale, int64_t lead,
-    int64_t rows, int cols) {
-  const int lane = threadIdx.x & 63;
-  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (r >= lead * rows) return;
-  const int64_t l = r / rows, i = r - l * rows;
-  const T* src = x + l * xsl + i * xsr;
-  int8_t* dst = q + l * qsl + i * qsr;
+__device__ __forceinline__ void row_at(const Rows& p, uint32_t r,
+                                       const T** src, int8_t** dst) {
+  uint32_t l = 0, i = r;
+  if (p.lead > 1) {
+    l = r / p.rows;
+    i = r - l * p.rows;
+  }
+  *src = (const T*)p.x + l * p.xsl + i * p.xsr;
+  *dst = p.q + l * p.qsl + i * p.qsr;
+}
+
+// the V values at k, 0 behind the row
+template <typename T, int V>
+__device__ __forceinline__ void load_piece(const T* src, int k, int cols,
+                                           float (&v)[V]) {
+  if (k + V <= cols) {
+    const auto t = *reinterpret_cast<const Vec<T, V>*>(src + k);
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = to_f32(t.v[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = k + j < cols ? to_f32(src[k + j]) : 0.f;
+  }
+}
+
+template <int V>
+__device__ __forceinline__ uint32_t top_of(const float (&v)[V]) {
   uint32_t top = 0;
-  for (int k = lane; k < cols; k += 64)
-    top = max(top, abs_bits(to_f32(src[k])));
+#pragma unroll
+  for (int j = 0; j < V; ++j) top = max(top, abs_bits(v[j]));
+  return top;
+}
+
+template <int V>
+__device__ __forceinline__ void store_piece(int8_t* dst, int k, int cols,
+                                            const float (&v)[V], RowScale rs) {
+  if (k >= cols) return;
+  Vec<uint8_t, V> o;
+#pragma unroll
+  for (int h = 0; h < V; h += 4) {
+    const float four[4] = {v[h], v[h + 1], v[h + 2], v[h + 3]};
+    const uint32_t word = row_codes(four, rs);
+    __builtin_memcpy(o.v + h, &word, 4);
+  }
+  if (k + V <= cols) {
+    *reinterpret_cast<Vec<uint8_t, V>*>(dst + k) = o;
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (k + j < cols) dst[k + j] = (int8_t)o.v[j];
+  }
+}
+
+// A row to 2^lbits lanes of a wave, R pieces of 16 bytes a lane.
+template <typename T, int R>
+__global__ __launch_bounds__(256) void wave_rows_kernel(Rows p, int lbits) {
+  constexpr int V = 16 / sizeof(T);
+  const int lane = threadIdx.x & 63, L = 1 << lbits;
+  const uint32_t r =
+      ((blockIdx.x * 4 + (threadIdx.x >> 6)) << (6 - lbits)) + (lane >> lbits);
+  const bool in = r < p.lead * p.rows;
+  const T* src;
+  int8_t* dst;
+  row_at<T>(p, in ? r : 0, &src, &dst);
+  const int cols = in ? p.cols : 0, k0 = (lane & (L - 1)) * V;
+  float v[R][V];
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    load_piece<T, V>(src, k0 + i * L * V, cols, v[i]);
+#pragma unroll
+  for (int i = 0; i < R; ++i) top = max(top, top_of<V>(v[i]));
+  for (int off = L >> 1; off > 0; off >>= 1)
+    top = max(top, (uint32_t)__shfl_xor((int)top, off));
+  const RowScale rs = row_scale(top);
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    store_piece<V>(dst, k0 + i * L * V, cols, v[i], rs);
+  if (in && k0 == 0) p.scale[r] = rs.scale;
+}
+
+// A row to a block: R pieces a thread in registers, what is longer is read
+// again for its codes.
+template <typename T, int R>
+__global__ __launch_bounds__(1024) void block_rows_kernel(Rows p) {
+  constexpr int V = 16 / sizeof(T);
+  __shared__ uint32_t tops[16];
+  const int tid = threadIdx.x, waves = blockDim.x >> 6;
+  const T* src;
+  int8_t* dst;
+  row_at<T>(p, blockIdx.x, &src, &dst);
+  const int k0 = tid * V, step = blockDim.x * V;
+  float v[R][V];
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    load_piece<T, V>(src, k0 + i * step, p.cols, v[i]);
+#pragma unroll
+  for (int i = 0; i < R; ++i) top = max(top, top_of<V>(v[i]));
+  for (int k = k0 + R * step; k < p.cols; k += step) {
+    float w[V];
+    load_piece<T, V>(src, k, p.cols, w);
+    top = max(top, top_of<V>(w));
+  }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1)
     top = max(top, (uint32_t)__shfl_xor((int)top, off));
+  if ((tid & 63) == 0) tops[tid >> 6] = top;
+  __syncthreads();
+  for (int w = 0; w < waves; ++w) top = max(top, tops[w]);
   const RowScale rs = row_scale(top);
-  for (int k = lane; k < cols; k += 64)
-    dst[k] = (int8_t)row_code(to_f32(src[k]), rs);
-  if (lane == 0) scale[r] = rs.scale;
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    store_piece<V>(dst, k0 + i * step, p.cols, v[i], rs);
+  for (int k = k0 + R * step; k < p.cols; k += step) {
+    float w[V];
+    load_piece<T, V>(src, k, p.cols, w);
+    store_piece<V>(dst, k, p.cols, w, rs);
+  }
+  if (tid == 0) p.scale[blockIdx.x] = rs.scale;
 }
 
+template <typename T, int R>
+void launch_waves(const Rows& p, int lbits, hipStream_t stream) {
+  const uint32_t rows = p.lead * p.rows, per = 4u << (6 - lbits);
+  hipLaunchKernelGGL((wave_rows_kernel<T, R>), dim3((rows + per - 1) / per),
+                     dim3(256), 0, stream, p, lbits);
+}
+
+// Waves take rows of up to 64 values a lane, where there are rows for all of
+// the chip's units; blocks take longer ones, and fewer.
 template <typename T>
-void launch(const void* x, int64_t xsl, int64_t xsr, int8_t* q, int64_t qsl,
-            int64_t qsr, float* scale, int64_t lead, int64_t rows, int cols,
-            hipStream_t stream) {
-  const int64_t blocks = (lead * rows + 3) / 4;
-  hipLaunchKernelGGL(quantize_rows_kernel<T>, dim3((uint32_t)blocks),
-                     dim3(256), 0, stream, (const T*)x, xsl, xsr, q, qsl, qsr,
-                     scale, lead, rows, cols);
+void choose(const Rows& p, hipStream_t stream) {
+  constexpr int V = 16 / sizeof(T);
+  const int64_t pieces = ((int64_t)p.cols + V - 1) / V;
+  const uint32_t rows = p.lead * p.rows;
+  if (pieces * V > 4096 || (pieces > 64 && rows < 1024)) {
+    const int threads =
+        (int)std::min<int64_t>(1024, (pieces + 63) / 64 * 64);
+    hipLaunchKernelGGL((block_rows_kernel<T, 2>), dim3(rows), dim3(threads), 0,
+                       stream, p);
+    return;
+  }
+  int lbits = 0;
+  while (lbits < 6 && (1 << lbits) < pieces) ++lbits;
+  const int64_t turns = (pieces + 63) / 64;
+  if (turns <= 1) launch_waves<T, 1>(p, lbits, stream);
+  else if (turns <= 2) launch_waves<T, 2>(p, lbits, stream);
+  else if (turns <= 4) launch_waves<T, 4>(p, lbits, stream);
+  else if (turns <= 8) launch_waves<T, 8>(p, lbits, stream);
+  else launch_waves<T, 64 / V>(p, lbits, stream);
 }
 
 }  // namespace
@@ -46,11 +182,9 @@ extern "C" void des_launch_quantize_rows(const void* x, int elem, int64_t xsl,
                                          int64_t qsr, float* scale,
                                          int64_t lead, int64_t rows, int cols,
                                          hipStream_t stream) {
-  if (elem == ELEM_F32)
-    launch<float>(x, xsl, xsr, q, qsl, qsr, scale, lead, rows, cols, stream);
-  else if (elem == ELEM_BF16)
-    launch<Bf16>(x, xsl, xsr, q, qsl, qsr, scale, lead, rows, cols, stream);
-  else
-    launch<_Float16>(x, xsl, xsr, q, qsl, qsr, scale, lead, rows, cols,
-                     stream);
+  const Rows p = {x,   q,   scale,          xsl,            xsr,
+                  qsl, qsr, (uint32_t)lead, (uint32_t)rows, cols};
+  if (elem == ELEM_F32) choose<float>(p, stream);
+  else if (elem == ELEM_BF16) choose<Bf16>(p, stream);
+  else choose<_Float16>(p, stream);
 }
