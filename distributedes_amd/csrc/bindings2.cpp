@@ -32,6 +32,8 @@ void des_launch_square_sums(const DesClipTable*, int64_t, double*,
 void des_launch_norm(const double*, int, float*, hipStream_t);
 void des_launch_clip_scale(const DesClipTable*, int64_t, const double*, int,
                            double, float*, bool, hipStream_t);
+void des_launch_clip_small(const DesClipTable*, double, float*, bool,
+                           hipStream_t);
 }
 
 namespace {
@@ -424,14 +426,22 @@ void check_tensors(const std::vector<Tensor>& tensors) {
   }
 }
 
-// A share of a tensor is one block's work: 2^14 values, or more where that
-// would give over 2048 blocks (each block of the second pass joins all sums).
+// A share of a tensor is one block's work: 2^12 values, or more where that
+// would give over 1024 blocks (each block of the second pass joins all sums).
 int64_t share_of(const std::vector<Tensor>& tensors) {
   int64_t total = 0;
   for (const Tensor& t : tensors) total += t.numel();
   int64_t share = 1 << 12;
-  while (total / share > 2048) share *= 2;
+  while (total / share > 1024) share *= 2;
   return share;
+}
+
+// Few values in few tensors: one block does it all in one launch.
+bool is_small(const std::vector<Tensor>& tensors) {
+  if (tensors.size() > 32) return false;
+  int64_t total = 0;
+  for (const Tensor& t : tensors) total += t.numel();
+  return total <= 1 << 15;
 }
 
 struct Tables {
@@ -481,8 +491,14 @@ Tensor global_norm(const std::vector<Tensor>& tensors) {
   for (const Tensor& t : tensors) in.push_back(t.contiguous());
   const int64_t share = share_of(in);
   const Tables tables = tables_of(in, {}, share);
-  const Tensor sums = square_sums(tables, share, in[0]);
   Tensor norm = at::empty({}, in[0].options().dtype(at::kFloat));
+  if (is_small(in)) {
+    des_launch_clip_small(&tables.tables[0], 0.0, norm.data_ptr<float>(),
+                          false, cur_stream());
+    CHECK_LAUNCH();
+    return norm;
+  }
+  const Tensor sums = square_sums(tables, share, in[0]);
   des_launch_norm(sums.data_ptr<double>(), (int)tables.blocks,
                   norm.data_ptr<float>(), cur_stream());
   CHECK_LAUNCH();
@@ -538,8 +554,14 @@ std::pair<std::vector<Tensor>, Tensor> clip_by_global_norm(
   }
   const int64_t share = share_of(in);
   const Tables tables = tables_of(in, to, share);
-  const Tensor sums = square_sums(tables, share, in[0]);
   Tensor norm = at::empty({}, in[0].options().dtype(at::kFloat));
+  if (is_small(in)) {
+    des_launch_clip_small(&tables.tables[0], max_norm, norm.data_ptr<float>(),
+                          true, cur_stream());
+    CHECK_LAUNCH();
+    return {to, norm};
+  }
+  const Tensor sums = square_sums(tables, share, in[0]);
   bool first = true;
   for (const DesClipTable& t : tables.tables) {
     des_launch_clip_scale(&t, share, sums.data_ptr<double>(),

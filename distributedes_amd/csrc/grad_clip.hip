@@ -10,12 +10,20 @@
 #include "grad_clip.h"
 #include "int8.h"
 
+//
+// Memory bound: the tensors are read for the norm and once more to be scaled,
+// since no value can be written before the last is read.  The second pass goes
+// over them backwards: what the first read last is still in the caches.
+#include <algorithm>
+
 namespace {
 
 using namespace des;
 
 constexpr int THREADS = 256;
+constexpr int SMALL = 1024;  // threads of the block that does all by itself
 
+template <int T>
 __device__ __forceinline__ double block_sum(double v, double* red) {
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
@@ -23,7 +31,8 @@ __device__ __forceinline__ double block_sum(double v, double* red) {
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
   double s = 0.0;
-  for (int i = 0; i < (int)blockDim.x / 64; ++i) s += red[i];
+#pragma unroll
+  for (int i = 0; i < T / 64; ++i) s += red[i];
   return s;
 }
 
@@ -37,15 +46,70 @@ __device__ __forceinline__ int tensor_of(const DesClipTable& t, int b) {
   return lo;
 }
 
-template <typename T>
+// [begin, end) of a tensor, in pieces of 16 bytes at any address, four under
+// way a thread
+template <typename T, int N>
 __device__ double share_sum(const void* in, int64_t begin, int64_t end) {
+  constexpr int V = 16 / sizeof(T);
   const T* p = (const T*)in;
-  double s = 0.0;
-  for (int64_t i = begin + threadIdx.x; i < end; i += THREADS) {
-    const double v = (double)to_f32(p[i]);
-    s += v * v;
+  double s[V] = {};
+  int64_t i = begin + threadIdx.x * V;
+#pragma unroll 4
+  for (; i + V <= end; i += N * V) {
+    const auto t = *reinterpret_cast<const Vec<T, V>*>(p + i);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const double v = (double)to_f32(t.v[j]);
+      s[j] = fma(v, v, s[j]);
+    }
   }
-  return s;
+  for (; i < end; ++i) {  // one thread has a piece that is cut short
+    const double v = (double)to_f32(p[i]);
+    s[0] = fma(v, v, s[0]);
+  }
+  double all = 0.0;
+#pragma unroll
+  for (int j = 0; j < V; ++j) all += s[j];
+  return all;
+}
+
+template <typename T, int N>
+__device__ void share_scale(const void* in, void* out, int64_t begin,
+                            int64_t end, double c) {
+  constexpr int V = 16 / sizeof(T);
+  const T* p = (const T*)in;
+  T* o = (T*)out;
+  int64_t i = begin + threadIdx.x * V;
+#pragma unroll 4
+  for (; i + V <= end; i += N * V) {
+    const auto t = *reinterpret_cast<const Vec<T, V>*>(p + i);
+    Vec<T, V> r;
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      r.v[j] = from_f32<T>((float)((double)to_f32(t.v[j]) * c));
+    *reinterpret_cast<Vec<T, V>*>(o + i) = r;
+  }
+  for (; i < end; ++i) o[i] = from_f32<T>((float)((double)to_f32(p[i]) * c));
+}
+
+template <int N>
+__device__ double any_sum(const DesClipTable& t, int i, int64_t begin,
+                          int64_t end) {
+  if (t.elem[i] == ELEM_F32) return share_sum<float, N>(t.in[i], begin, end);
+  if (t.elem[i] == ELEM_BF16) return share_sum<Bf16, N>(t.in[i], begin, end);
+  return share_sum<_Float16, N>(t.in[i], begin, end);
+}
+
+template <int N>
+__device__ void any_scale(const DesClipTable& t, int i, int64_t begin,
+                          int64_t end, double c) {
+  if (c == 1.0 && t.in[i] == t.out[i]) return;  // in place, nothing to do
+  if (t.elem[i] == ELEM_F32)
+    share_scale<float, N>(t.in[i], t.out[i], begin, end, c);
+  else if (t.elem[i] == ELEM_BF16)
+    share_scale<Bf16, N>(t.in[i], t.out[i], begin, end, c);
+  else
+    share_scale<_Float16, N>(t.in[i], t.out[i], begin, end, c);
 }
 
 __global__ __launch_bounds__(THREADS) void square_sums_kernel(
@@ -54,18 +118,15 @@ __global__ __launch_bounds__(THREADS) void square_sums_kernel(
   const int b = blockIdx.x, i = tensor_of(t, b);
   const int64_t begin = (b - t.first[i]) * share;
   const int64_t end = min(begin + share, t.numel[i]);
-  const double s = t.elem[i] == ELEM_F32 ? share_sum<float>(t.in[i], begin, end)
-                   : t.elem[i] == ELEM_BF16
-                       ? share_sum<Bf16>(t.in[i], begin, end)
-                       : share_sum<_Float16>(t.in[i], begin, end);
-  const double all = block_sum(s, red);
+  const double all =
+      block_sum<THREADS>(any_sum<THREADS>(t, i, begin, end), red);
   if (threadIdx.x == 0) sums[b] = all;
 }
 
 __device__ double norm_of(const double* sums, int n, double* red) {
   double s = 0.0;
   for (int i = threadIdx.x; i < n; i += THREADS) s += sums[i];
-  return sqrt(block_sum(s, red));
+  return sqrt(block_sum<THREADS>(s, red));
 }
 
 __global__ __launch_bounds__(THREADS) void norm_kernel(
@@ -73,15 +134,6 @@ __global__ __launch_bounds__(THREADS) void norm_kernel(
   __shared__ double red[THREADS / 64];
   const double v = norm_of(sums, n, red);
   if (threadIdx.x == 0) *norm = (float)v;
-}
-
-template <typename T>
-__device__ void share_scale(const void* in, void* out, int64_t begin,
-                            int64_t end, double c) {
-  const T* p = (const T*)in;
-  T* o = (T*)out;
-  for (int64_t i = begin + threadIdx.x; i < end; i += THREADS)
-    o[i] = from_f32<T>((float)((double)to_f32(p[i]) * c));
 }
 
 // Every block joins the sums by itself, in the same order: cheaper than a
@@ -92,16 +144,25 @@ __global__ __launch_bounds__(THREADS) void scale_kernel(
   __shared__ double red[THREADS / 64];
   const double v = norm_of(sums, n, red);
   const double c = v > max_norm ? max_norm / v : 1.0;
-  const int b = blockIdx.x, i = tensor_of(t, b);
-  if (write_norm && b == 0 && threadIdx.x == 0) *norm = (float)v;
+  if (write_norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)v;
+  const int b = gridDim.x - 1 - blockIdx.x, i = tensor_of(t, b);
   const int64_t begin = (b - t.first[i]) * share;
-  const int64_t end = min(begin + share, t.numel[i]);
-  if (t.elem[i] == ELEM_F32)
-    share_scale<float>(t.in[i], t.out[i], begin, end, c);
-  else if (t.elem[i] == ELEM_BF16)
-    share_scale<Bf16>(t.in[i], t.out[i], begin, end, c);
-  else
-    share_scale<_Float16>(t.in[i], t.out[i], begin, end, c);
+  any_scale<THREADS>(t, i, begin, min(begin + share, t.numel[i]), c);
+}
+
+// Norm and scaling of a few small tensors by one block.
+__global__ __launch_bounds__(SMALL) void small_kernel(DesClipTable t,
+                                                      double max_norm,
+                                                      float* __restrict__ norm,
+                                                      bool scale) {
+  __shared__ double red[SMALL / 64];
+  double s = 0.0;
+  for (int i = 0; i < t.count; ++i) s += any_sum<SMALL>(t, i, 0, t.numel[i]);
+  const double v = sqrt(block_sum<SMALL>(s, red));
+  if (threadIdx.x == 0) *norm = (float)v;
+  if (!scale) return;
+  const double c = v > max_norm ? max_norm / v : 1.0;
+  for (int i = 0; i < t.count; ++i) any_scale<SMALL>(t, i, 0, t.numel[i], c);
 }
 
 }  // namespace
@@ -125,4 +186,11 @@ extern "C" void des_launch_clip_scale(const DesClipTable* t, int64_t share,
   hipLaunchKernelGGL(scale_kernel, dim3((uint32_t)t->first[t->count]),
                      dim3(THREADS), 0, stream, *t, share, sums, n, max_norm,
                      norm, write_norm);
+}
+
+extern "C" void des_launch_clip_small(const DesClipTable* t, double max_norm,
+                                      float* norm, bool scale,
+                                      hipStream_t stream) {
+  hipLaunchKernelGGL(small_kernel, dim3(1), dim3(SMALL), 0, stream, *t,
+                     max_norm, norm, scale);
 }

@@ -33,36 +33,36 @@ __device__ __forceinline__ void row_at(const Rows& p, uint32_t r,
   *dst = p.q + l * p.qsl + i * p.qsr;
 }
 
-// the V values at k, 0 behind the row
+// the V values at k, 0 behind the row, in their own type: half the registers
+// for 16-bit rows, so that twice the loads are under way
 template <typename T, int V>
-__device__ __forceinline__ void load_piece(const T* src, int k, int cols,
-                                           float (&v)[V]) {
-  if (k + V <= cols) {
-    const auto t = *reinterpret_cast<const Vec<T, V>*>(src + k);
+__device__ __forceinline__ Vec<T, V> load_piece(const T* src, int k,
+                                                int cols) {
+  if (k + V <= cols) return *reinterpret_cast<const Vec<T, V>*>(src + k);
+  Vec<T, V> t = {};
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = to_f32(t.v[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = k + j < cols ? to_f32(src[k + j]) : 0.f;
-  }
+  for (int j = 0; j < V; ++j)
+    if (k + j < cols) t.v[j] = src[k + j];
+  return t;
 }
 
-template <int V>
-__device__ __forceinline__ uint32_t top_of(const float (&v)[V]) {
+template <typename T, int V>
+__device__ __forceinline__ uint32_t top_of(const Vec<T, V>& t) {
   uint32_t top = 0;
 #pragma unroll
-  for (int j = 0; j < V; ++j) top = max(top, abs_bits(v[j]));
+  for (int j = 0; j < V; ++j) top = max(top, abs_bits(to_f32(t.v[j])));
   return top;
 }
 
-template <int V>
+template <typename T, int V>
 __device__ __forceinline__ void store_piece(int8_t* dst, int k, int cols,
-                                            const float (&v)[V], RowScale rs) {
+                                            const Vec<T, V>& t, RowScale rs) {
   if (k >= cols) return;
   Vec<uint8_t, V> o;
 #pragma unroll
   for (int h = 0; h < V; h += 4) {
-    const float four[4] = {v[h], v[h + 1], v[h + 2], v[h + 3]};
+    const float four[4] = {to_f32(t.v[h]), to_f32(t.v[h + 1]),
+                           to_f32(t.v[h + 2]), to_f32(t.v[h + 3])};
     const uint32_t word = row_codes(four, rs);
     __builtin_memcpy(o.v + h, &word, 4);
   }
@@ -87,19 +87,18 @@ __global__ __launch_bounds__(256) void wave_rows_kernel(Rows p, int lbits) {
   int8_t* dst;
   row_at<T>(p, in ? r : 0, &src, &dst);
   const int cols = in ? p.cols : 0, k0 = (lane & (L - 1)) * V;
-  float v[R][V];
+  Vec<T, V> v[R];
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < R; ++i)
-    load_piece<T, V>(src, k0 + i * L * V, cols, v[i]);
+  for (int i = 0; i < R; ++i) v[i] = load_piece<T, V>(src, k0 + i * L * V, cols);
 #pragma unroll
-  for (int i = 0; i < R; ++i) top = max(top, top_of<V>(v[i]));
+  for (int i = 0; i < R; ++i) top = max(top, top_of(v[i]));
   for (int off = L >> 1; off > 0; off >>= 1)
     top = max(top, (uint32_t)__shfl_xor((int)top, off));
   const RowScale rs = row_scale(top);
 #pragma unroll
   for (int i = 0; i < R; ++i)
-    store_piece<V>(dst, k0 + i * L * V, cols, v[i], rs);
+    store_piece(dst, k0 + i * L * V, cols, v[i], rs);
   if (in && k0 == 0) p.scale[r] = rs.scale;
 }
 
@@ -114,17 +113,14 @@ __global__ __launch_bounds__(1024) void block_rows_kernel(Rows p) {
   int8_t* dst;
   row_at<T>(p, blockIdx.x, &src, &dst);
   const int k0 = tid * V, step = blockDim.x * V;
-  float v[R][V];
+  Vec<T, V> v[R];
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < R; ++i)
-    load_piece<T, V>(src, k0 + i * step, p.cols, v[i]);
+  for (int i = 0; i < R; ++i) v[i] = load_piece<T, V>(src, k0 + i * step, p.cols);
 #pragma unroll
-  for (int i = 0; i < R; ++i) top = max(top, top_of<V>(v[i]));
+  for (int i = 0; i < R; ++i) top = max(top, top_of(v[i]));
   for (int k = k0 + R * step; k < p.cols; k += step) {
-    float w[V];
-    load_piece<T, V>(src, k, p.cols, w);
-    top = max(top, top_of<V>(w));
+    top = max(top, top_of(load_piece<T, V>(src, k, p.cols)));
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1)
@@ -135,11 +131,9 @@ __global__ __launch_bounds__(1024) void block_rows_kernel(Rows p) {
   const RowScale rs = row_scale(top);
 #pragma unroll
   for (int i = 0; i < R; ++i)
-    store_piece<V>(dst, k0 + i * step, p.cols, v[i], rs);
+    store_piece(dst, k0 + i * step, p.cols, v[i], rs);
   for (int k = k0 + R * step; k < p.cols; k += step) {
-    float w[V];
-    load_piece<T, V>(src, k, p.cols, w);
-    store_piece<V>(dst, k, p.cols, w, rs);
+    store_piece(dst, k, p.cols, load_piece<T, V>(src, k, p.cols), rs);
   }
   if (tid == 0) p.scale[blockIdx.x] = rs.scale;
 }
