@@ -31,8 +31,8 @@ void des_launch_square_sums(const DesClipTable*, int64_t, double*,
                             hipStream_t);
 void des_launch_norm(const double*, int, float*, hipStream_t);
 void des_launch_clip_scale(const DesClipTable*, int64_t, const double*, int,
-                           double, float*, bool, hipStream_t);
-void des_launch_clip_small(const DesClipTable*, double, float*, bool,
+                           double, float*, bool, bool, hipStream_t);
+void des_launch_clip_small(const DesClipTable*, int64_t, double, float*, bool,
                            hipStream_t);
 }
 
@@ -426,22 +426,26 @@ void check_tensors(const std::vector<Tensor>& tensors) {
   }
 }
 
-// A share of a tensor is one block's work: 2^12 values, or more where that
-// would give over 1024 blocks (each block of the second pass joins all sums).
-int64_t share_of(const std::vector<Tensor>& tensors) {
+int64_t total_of(const std::vector<Tensor>& tensors) {
   int64_t total = 0;
   for (const Tensor& t : tensors) total += t.numel();
-  int64_t share = 1 << 12;
-  while (total / share > 1024) share *= 2;
-  return share;
+  return total;
 }
 
 // Few values in few tensors: one block does it all in one launch.
 bool is_small(const std::vector<Tensor>& tensors) {
-  if (tensors.size() > 32) return false;
-  int64_t total = 0;
-  for (const Tensor& t : tensors) total += t.numel();
-  return total <= 1 << 15;
+  return tensors.size() <= 32 && total_of(tensors) <= 1 << 15;
+}
+
+// A share of a tensor is one block's work (a wave's, where it is small): 2^12
+// values, or more where that would give over 2048 blocks, since each block of
+// the second pass joins all sums.
+int64_t share_of(const std::vector<Tensor>& tensors) {
+  if (is_small(tensors)) return 1 << 10;
+  const int64_t total = total_of(tensors);
+  int64_t share = 1 << 12;
+  while (total / share > 2048) share *= 2;
+  return share;
 }
 
 struct Tables {
@@ -493,8 +497,8 @@ Tensor global_norm(const std::vector<Tensor>& tensors) {
   const Tables tables = tables_of(in, {}, share);
   Tensor norm = at::empty({}, in[0].options().dtype(at::kFloat));
   if (is_small(in)) {
-    des_launch_clip_small(&tables.tables[0], 0.0, norm.data_ptr<float>(),
-                          false, cur_stream());
+    des_launch_clip_small(&tables.tables[0], share, 0.0,
+                          norm.data_ptr<float>(), false, cur_stream());
     CHECK_LAUNCH();
     return norm;
   }
@@ -556,17 +560,20 @@ std::pair<std::vector<Tensor>, Tensor> clip_by_global_norm(
   const Tables tables = tables_of(in, to, share);
   Tensor norm = at::empty({}, in[0].options().dtype(at::kFloat));
   if (is_small(in)) {
-    des_launch_clip_small(&tables.tables[0], max_norm, norm.data_ptr<float>(),
-                          true, cur_stream());
+    des_launch_clip_small(&tables.tables[0], share, max_norm,
+                          norm.data_ptr<float>(), true, cur_stream());
     CHECK_LAUNCH();
     return {to, norm};
   }
   const Tensor sums = square_sums(tables, share, in[0]);
   bool first = true;
+  int64_t bytes = 0;
+  for (const Tensor& t : in) bytes += t.nbytes();
   for (const DesClipTable& t : tables.tables) {
     des_launch_clip_scale(&t, share, sums.data_ptr<double>(),
                           (int)tables.blocks, max_norm,
-                          norm.data_ptr<float>(), first, cur_stream());
+                          norm.data_ptr<float>(), first, bytes > 32 << 20,
+                          cur_stream());
     CHECK_LAUNCH();
     first = false;
   }

@@ -2,8 +2,7 @@
 // the definition).
 //
 // Memory bound: a row is read once and held in registers between its maximum
-// and its codes.  About 6 operations a value (see row_codes) are 2 to 4 times
-// less than the loads take.
+// and its codes, about 6 operations a value (see row_codes).
 #include <algorithm>
 
 #include "int8.h"
@@ -145,28 +144,38 @@ void launch_waves(const Rows& p, int lbits, hipStream_t stream) {
                      dim3(256), 0, stream, p, lbits);
 }
 
-// Waves take rows of up to 64 values a lane, where there are rows for all of
-// the chip's units; blocks take longer ones, and fewer.
+// Pieces of 16 bytes and who takes them; measured:
+//  - up to 256 a row: lanes of a wave, three or four pieces each, and as many rows
+//    a wave as fit. 262144 x 256 fp32 by 64 lanes 73.8 us, 32 60.0, 16 62.4, 8
+//    71.0; 10000 x 376 fp32 by 64 6.1, 32 6.0, 16 6.4.
+//  - longer rows: a block, four pieces a thread. 8192 x 3136 bf16 by 128 threads
+//    15.1 us, 256 15.4, 448 24.6, a wave 17.5.
+//  - few rows: a block, a piece a thread, for latency. 16 x 3136 bf16 by 448
+//    threads 4.2 us, 256 6.1.
 template <typename T>
 void choose(const Rows& p, hipStream_t stream) {
   constexpr int V = 16 / sizeof(T);
   const int64_t pieces = ((int64_t)p.cols + V - 1) / V;
   const uint32_t rows = p.lead * p.rows;
-  if (pieces * V > 4096 || (pieces > 64 && rows < 1024)) {
-    const int threads =
-        (int)std::min<int64_t>(1024, (pieces + 63) / 64 * 64);
-    hipLaunchKernelGGL((block_rows_kernel<T, 2>), dim3(rows), dim3(threads), 0,
-                       stream, p);
+  auto threads = [](int64_t n) {
+    return dim3((uint32_t)std::min<int64_t>(1024, (n + 63) / 64 * 64));
+  };
+  if (pieces > 64 && rows < 512) {
+    hipLaunchKernelGGL((block_rows_kernel<T, 1>), dim3(rows), threads(pieces),
+                       0, stream, p);
+    return;
+  }
+  if (pieces > 256) {
+    hipLaunchKernelGGL((block_rows_kernel<T, 4>), dim3(rows),
+                       threads((pieces + 3) / 4), 0, stream, p);
     return;
   }
   int lbits = 0;
-  while (lbits < 6 && (1 << lbits) < pieces) ++lbits;
-  const int64_t turns = (pieces + 63) / 64;
+  while (lbits < 6 && (4 << lbits) < pieces) ++lbits;
+  const int64_t turns = (pieces + (1 << lbits) - 1) >> lbits;
   if (turns <= 1) launch_waves<T, 1>(p, lbits, stream);
   else if (turns <= 2) launch_waves<T, 2>(p, lbits, stream);
-  else if (turns <= 4) launch_waves<T, 4>(p, lbits, stream);
-  else if (turns <= 8) launch_waves<T, 8>(p, lbits, stream);
-  else launch_waves<T, 64 / V>(p, lbits, stream);
+  else launch_waves<T, 4>(p, lbits, stream);
 }
 
 }  // namespace
