@@ -72,11 +72,7 @@ def evaluate(checkpoint_or_state, config: Optional[Config] = None,
         state.load_payload(load_checkpoint(checkpoint_or_state))
 
     P = episodes
-    dt = (torch.bfloat16 if state.device.type == "cuda"
-          and state.cfg.precision == "bf16" else torch.float32)
-    stride = ((state.dim + 7) & ~7) if state._hip_rollout is not None else state.dim
-    pop_w = torch.zeros(P, stride, dtype=dt, device=state.device)
-    pop_w[:, :state.dim] = state.theta.to(dt)
+    pop_w = state.one_policy(P)
     # scoped eval: explicit env ids (one distinct stream per episode — the
     # training slice would pair-share streams under antithetic sampling) and
     # observe=False so eval observations never enter the normalizer deltas.

@@ -31,6 +31,7 @@ class Config:
     adam_beta1: float = 0.9
     adam_beta2: float = 0.999
     adam_eps: float = 1e-8
+    max_grad_norm: float = 0.0       # bound on the descent direction's norm; 0 = none
 
     # --- CEM ---
     elite_frac: float = 0.2
@@ -54,6 +55,8 @@ class Config:
     device: str = "auto"             # auto | cuda | cpu
     backend: Optional[str] = None    # None=auto: nccl if cuda else gloo
     precision: str = "bf16"          # population forward dtype on GPU: bf16 | fp32
+                                     # int8 (mlp, any device): layers in 8 bits,
+                                     # one scale a channel and observation
     overlap_comm: bool = True        # side-stream overlap of collectives (GPU)
     use_hip_graphs: bool = True      # capture the rollout loop in a hipGraph
 
@@ -78,6 +81,14 @@ class Config:
             raise ValueError(f"unknown algo {self.algo!r}")
         if self.rank_shaping not in ("centered", "normalized", "raw"):
             raise ValueError(f"unknown rank_shaping {self.rank_shaping!r}")
+        if self.precision == "int8" and self.model != "mlp":
+            raise ValueError("precision 'int8' needs model 'mlp', not "
+                             f"{self.model!r}")
+        if not self.max_grad_norm >= 0:
+            raise ValueError("max_grad_norm must be at least 0")
+        if self.max_grad_norm and self.algo != "es":
+            raise ValueError("max_grad_norm bounds the ES gradient estimate; "
+                             f"algo {self.algo!r} has none")
         return self
 
 

@@ -30,7 +30,7 @@ import torch
 
 from ..config import Config
 from ..envs import make_env
-from ..models import make_model
+from ..models import Int8Layers, make_model
 from ..parallel import Comm
 from ..utils import (IdentityNormalizer, MetricsLogger, RunningNormalizer,
                      save_checkpoint)
@@ -121,6 +121,8 @@ class TrainState:
         self.metrics = MetricsLogger(cfg.metrics_path, rank=self.rank,
                                      log_every=cfg.log_every)
         self._pop_w = None          # reusable [local_pop, D] perturbed weights
+        self._flat_w = None         # precision int8: the fp32 rows behind them
+        self.grad_norm = None       # of the last update (max_grad_norm > 0)
         self._offs_cache = {}       # generation -> (offsets, signs) prefetch
 
         # GPU-native rollout path (K3/K5/K7/K8 kernels); torch loop otherwise
@@ -212,7 +214,22 @@ class TrainState:
         return fitness, P * steps_done, float(ep_len.mean())
 
     def pop_forward(self, pop_w: torch.Tensor, obs: torch.Tensor) -> torch.Tensor:
+        if isinstance(pop_w, Int8Layers):
+            return self.model.pop_forward_int8(self.ops, pop_w, obs)
         return self.model.pop_forward_ref(pop_w, obs)
+
+    def one_policy(self, P: int):
+        """theta as the weights that rollout() takes, for P environments."""
+        if self.cfg.precision == "int8":
+            layers = Int8Layers(self.model, P, self.device, shared=True)
+            layers.load(self.ops, self.theta.unsqueeze(0))
+            return layers
+        dt = (torch.bfloat16 if self.device.type == "cuda"
+              and self.cfg.precision == "bf16" else torch.float32)
+        stride = ((self.dim + 7) & ~7) if self._hip_rollout is not None else self.dim
+        pop_w = torch.zeros(P, stride, dtype=dt, device=self.device)
+        pop_w[:, :self.dim] = self.theta.to(dt)
+        return pop_w
 
     # ------------------------------------------------------------------ #
     def perturb_local(self, offsets, signs) -> torch.Tensor:
@@ -221,6 +238,14 @@ class TrainState:
                      and self.device.type == "cuda") else torch.float32)
         base = self.theta
         sigma_vec = self.sigma_vec if cfg.algo == "cem" else None
+        if cfg.precision == "int8":
+            kw = {"out": self._flat_w} if self.ops.name == "hip" else {}
+            self._flat_w = self.ops.perturb(base, self.table, offsets, signs,
+                                            cfg.sigma, sigma_vec=sigma_vec, **kw)
+            if self._pop_w is None:
+                self._pop_w = Int8Layers(self.model, self.local_pop, self.device)
+            self._pop_w.load(self.ops, self._flat_w)
+            return self._pop_w
         kw = {}
         if self.ops.name == "hip":
             kw["pad_rows"] = self._hip_rollout is not None
@@ -253,6 +278,10 @@ class TrainState:
         self.comm.allreduce_(partial)                                # C4
         grad_ascent = partial / (cfg.pop * cfg.sigma)
         descent = cfg.weight_decay * self.theta - grad_ascent
+        if cfg.max_grad_norm:
+            # equal on every rank: so is the direction, after C4
+            _, self.grad_norm = self.ops.clip_by_global_norm(
+                [descent], cfg.max_grad_norm, out=[descent])
         self.optimizer.step(self.theta, descent)
         if (cfg.theta_allreduce_every
                 and (self.generation + 1) % cfg.theta_allreduce_every == 0):
@@ -383,6 +412,8 @@ def train_step(state: TrainState) -> dict:
         "ops_backend": state.ops.name,
         "hip_graphs": bool(getattr(state._hip_rollout, "last_used_graph", False)),
     }
+    if state.grad_norm is not None:
+        stats["grad_norm"] = float(state.grad_norm)   # before the bound
     ng = getattr(state.env, "n_games", 1)
     if ng > 1:
         # per-game fitness breakdown (BASELINE config #4: Atari-57 means 57

@@ -1,5 +1,5 @@
 from .base import ParamSpec, PolicyModel  # noqa: F401
-from .mlp import MLPPolicy  # noqa: F401
+from .mlp import Int8Layers, MLPPolicy  # noqa: F401
 from .nature_cnn import NatureCNNPolicy  # noqa: F401
 from .impala_cnn import ImpalaCNNPolicy  # noqa: F401
 

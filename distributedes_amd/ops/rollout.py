@@ -16,7 +16,8 @@ import torch
 
 log = logging.getLogger("distributedes_amd")
 
-from ..models import ImpalaCNNPolicy, MLPPolicy, NatureCNNPolicy
+from ..models import (ImpalaCNNPolicy, Int8Layers, MLPPolicy,
+                      NatureCNNPolicy)
 from ..models.base import ParamSpec
 
 
@@ -73,6 +74,9 @@ class HipRollout:
         self.ext = ext
         self.device = device
         self.P = None
+        if cfg.precision == "int8":
+            from .hip import HipOps
+            self._ops = HipOps()
         if isinstance(model, MLPPolicy):
             self.kind = "mlp"
             self.h1 = model.hidden_sizes[0]
@@ -192,7 +196,13 @@ class HipRollout:
     # ------------------------------------------------------------------ #
     def _forward(self, pop_w: torch.Tensor, normalizer, slot_newest: int):
         """One policy forward: obs buffers -> action buffers."""
-        if self.kind == "mlp":
+        if isinstance(pop_w, Int8Layers):
+            obs = self.st_state if self.env_name == "cartpole" else self.hu_s
+            if getattr(normalizer, "_mean", obs).device == obs.device:
+                obs = normalizer.normalize(obs)
+            act = self.actions_f if self.env.continuous else self.actions_i
+            act.copy_(self.model.pop_forward_int8(self._ops, pop_w, obs))
+        elif self.kind == "mlp":
             obs = self.st_state if self.env_name == "cartpole" else self.hu_s
             nmean = getattr(normalizer, "_mean", None)
             if nmean is not None and nmean.device != self.device:
