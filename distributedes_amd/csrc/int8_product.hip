@@ -554,80 +554,154 @@ __device__ __forceinline__ void wait_loads() {
                              ((N >> 4) << 14));
 }
 
-// Writes Q x 4 results: of tokens m[q], channels n .. n + 3 (`have` of them
-// within the row).
-template <int Q>
-__device__ __forceinline__ void put_rows(const DesInt8Product& p, int64_t b,
-                                         const int (&m)[Q], int n, int have,
-                                         const v4f (&v)[Q]) {
+// a wave's shared memory for 32 tokens x 32 NT results of 4 bytes
+constexpr int tile_room(int nt) { return 32 * (nt * 128 + 16); }
+
+// shared memory of a tile's stages, and of its end
+constexpr int tiled_room(int wn, int wm, int nt, int mt, int s) {
+  return std::max(s * 32 * (wn * nt + wm * mt) * 128, wn * wm * tile_room(nt));
+}
+
+// Results of a wave's NT x MT blocks of sums.  V = 8: the results have 16 bits
+// and are finished where the sums are; V = 4: floats go through shared memory,
+// the activation and the type come afterwards (32 bits, or tanh, whose code is
+// long and stands here once).
+template <int NT, int MT, int V>
+__device__ __forceinline__ void tile_end(const DesInt8Product& p, int64_t b,
+                                         const v16i (&acc)[NT][MT],
+                                         const float (&sx)[MT],
+                                         const float* sw, const float* bias,
+                                         int8_t* mine, int lane, int n0,
+                                         int m0) {
+  constexpr int SIZE = V == 8 ? 2 : 4;            // of a value in shared memory
+  constexpr int ROW = NT * 32 * SIZE + 16;        // bytes
+  constexpr int LANES = NT * 32 / V, TOKENS = 64 / LANES;
+  const int half = lane >> 5, row = lane & 31;
+  const int n = n0 + lane % LANES * V, have = p.N - n;
+  const bool relu = p.act == 1, bf16 = p.out == ELEM_BF16;
+#pragma unroll 1
+  for (int i = 0; i < MT; ++i) {
 #pragma unroll
-  for (int q = 0; q < Q; ++q) {
-    if (m[q] >= p.M || have <= 0) continue;
-    const int64_t at = (b * p.M + m[q]) * p.N + n;
-    if (have >= 4) {
-      if (p.out == ELEM_F32) {
-        Vec<float, 4> o = {{v[q][0], v[q][1], v[q][2], v[q][3]}};
-        reinterpret_cast<Vec<float, 4>*>(reinterpret_cast<float*>(p.y) + at)[0] = o;
-      } else {
-        Vec<uint16_t, 4> o;
+    for (int ii = 0; ii < MT; ++ii) {
+      if (i != ii) continue;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          o.v[e] = p.out == ELEM_BF16
-                       ? from_f32<Bf16>(v[q][e]).bits
-                       : __builtin_bit_cast(uint16_t, (_Float16)v[q][e]);
-        reinterpret_cast<Vec<uint16_t, 4>*>(reinterpret_cast<uint16_t*>(p.y) +
-                                            at)[0] = o;
-      }
-    } else {
-      put1(p, at, v[q][0]);
-      if (have > 1) put1(p, at + 1, v[q][1]);
-      if (have > 2) put1(p, at + 2, v[q][2]);
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int c = j * 32 + 8 * g + 4 * half;
+          const v4f s4 = *reinterpret_cast<const v4f*>(sw + c);
+          const v4f b4 = *reinterpret_cast<const v4f*>(bias + c);
+          v4f v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            v[e] = fmaf((float)acc[j][ii][4 * g + e] * sx[ii], s4[e], b4[e]);
+          int8_t* to = mine + row * ROW + c * SIZE;
+          if constexpr (V == 8) {
+            if (relu)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];
+            Vec<uint16_t, 4> o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              o.v[e] = bf16 ? from_f32<Bf16>(v[e]).bits
+                            : __builtin_bit_cast(uint16_t, (_Float16)v[e]);
+            __builtin_memcpy(__builtin_assume_aligned(to, 8), &o, 8);
+          } else {
+            *reinterpret_cast<v4f*>(to) = v;
+          }
+        }
     }
+    __builtin_amdgcn_wave_barrier();
+    const int8_t* from = mine + lane / LANES * ROW + lane % LANES * 16;
+    int m = m0 + i * 32 + lane / LANES;
+    int64_t at = (b * p.M + m) * p.N + n;
+#pragma unroll 1
+    for (int t = 0; t < 32; t += TOKENS) {
+      const v4i got = *reinterpret_cast<const v4i*>(from + t * ROW);
+      if (m < p.M && have > 0) {
+        if constexpr (V == 8) {
+          uint16_t* y = reinterpret_cast<uint16_t*>(p.y) + at;
+          if (have >= 8) {
+            __builtin_memcpy(y, &got, 16);
+          } else {
+            for (int e = 0; e < have; ++e) {
+              const int w = e < 2 ? got[0] : e < 4 ? got[1] : e < 6 ? got[2] : got[3];
+              y[e] = (uint16_t)(e & 1 ? (uint32_t)w >> 16 : w);
+            }
+          }
+        } else {
+          v4f v = __builtin_bit_cast(v4f, got);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (relu) v[e] = v[e] < 0.f ? 0.f : v[e];
+            if (p.act == 2) v[e] = tanhf(v[e]);
+          }
+          if (have >= 4 && p.out == ELEM_F32) {
+            __builtin_memcpy(reinterpret_cast<float*>(p.y) + at, &v, 16);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (e < have) put1(p, at + e, v[e]);
+          }
+        }
+      }
+      m += TOKENS;
+      at += (int64_t)TOKENS * p.N;
+    }
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
 // Many rows: a block has WN x WM waves, each with NT x MT blocks of 32 x 32
-// results (channels x tokens), and takes K in stages of BK codes through
+// results (channels x tokens), and takes K in stages of 128 codes through
 // shared memory, S stages in a ring: while one is multiplied, S - 1 are on
-// their way.  A stage's rows lie BK bytes apart; the 16-byte piece c of row r
-// is kept at place c ^ (r & 7) (BK = 64: two rows share the banks' 128 bytes,
-// c ^ (r / 2 & 3)), so that the 8 lanes that read together (8 rows, the same
-// piece) meet 8 different places.  Loads write lanes' pieces next to each
+// their way.
+//
+// A stage's rows lie 128 bytes apart; the 16-byte piece c of row r is kept at
+// place c ^ (r / 2 & 7), so that the 16 lanes that read together (16 rows, the
+// same piece) meet all 64 banks once.  Loads write lanes' pieces next to each
 // other, so the places are exchanged where the pieces are read from memory.
 //
 // v_mfma_i32_32x32x32_i8: a lane gives 16 codes of row (lane & 31) at
 // k = 16 * (lane >> 5), and holds the results of token (lane & 31) for channels
 // 8 * (i / 4) + 4 * (lane >> 5) + i % 4, i < 16.
 //
-// The end is kept short: every instruction of a kernel comes from memory once a
-// launch, and 10 KB of unrolled epilogue took 10 us.
-template <int WN, int WM, int NT, int MT, int BK, int S>
+// What bounds it: with 256 x 256 results a block, the matrix units' power (2.1
+// POPS on values as they occur, 5.0 by their clock); with fewer results the
+// reads of both operands, 20 bytes a clock and unit, and the barriers of a
+// stage.  Tried without gain: K shared by two groups of waves in a block, four
+// stages, priorities around the products.
+template <int WN, int WM, int NT, int MT, int S>
 __global__ __launch_bounds__(64 * WN * WM) void tiled_kernel(
-    DesInt8Product p, uint32_t nblocks, uint32_t mblocks) {
+    DesInt8Product p, uint32_t nblocks, uint32_t mblocks, bool together) {
   constexpr int THREADS = 64 * WN * WM;
-  constexpr int BN = 32 * WN * NT, BM = 32 * WM * MT;
-  constexpr int ROW_PIECES = BK / 16;
-  constexpr int PIECES = (BN + BM) * ROW_PIECES / THREADS;  // a thread's
+  constexpr int BN = 32 * WN * NT, BM = 32 * WM * MT, BK = 128;
+  constexpr int PIECES = (BN + BM) * (BK / 16) / THREADS;  // a thread's
   constexpr int STAGE = (BN + BM) * BK;
+  constexpr int STEPS = BK / 32;
   extern __shared__ __align__(16) int8_t shared[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wn = wave % WN, wm = wave / WN;
   uint32_t id = blockIdx.x;
+  if (together) {  // blocks in turn go to 8 dies: each takes a piece of the list
+    const uint32_t each = gridDim.x / 8;
+    if (id < 8 * each) id = (id & 7) * each + (id >> 3);
+  }
   const int nb = id % nblocks;
   id /= nblocks;
   const int mb = id % mblocks;
   const int64_t b = id / mblocks;
   const int n0 = nb * BN, m0 = mb * BM;
-  auto place = [](int r) { return BK == 128 ? r & 7 : r >> 1 & 3; };
+  auto place = [](int r) { return r >> 1 & 7; };
 
   // a thread's pieces of a stage: rows of weights, then rows of tokens
   const int8_t* src[PIECES];
   int col[PIECES];
 #pragma unroll
   for (int i = 0; i < PIECES; ++i) {
-    const int at = i * THREADS + tid, r = at / ROW_PIECES;
-    col[i] = ((at % ROW_PIECES) ^ place(r)) * 16;
+    const int at = i * THREADS + tid, r = at >> 3;
+    col[i] = ((at & 7) ^ place(r)) * 16;
     src[i] = r < BN ? p.w + b * p.wsb + (int64_t)min(n0 + r, p.N - 1) * p.wsr
                     : p.x + b * p.xsb +
                           (int64_t)min(m0 + r - BN, p.M - 1) * p.xsr;
@@ -643,24 +717,30 @@ __global__ __launch_bounds__(64 * WN * WM) void tiled_kernel(
   };
 
   const int half = lane >> 5, row = lane & 31;
-  // the factors: a lane's token here, its four channels in the epilogue
-  constexpr int LANES = NT * 8, TOKENS = 64 / LANES;  // of one turn there
-  const int n = n0 + wn * NT * 32 + lane % LANES * 4;
-  const int have = p.N - n;
-  float sx[MT], sw[4], bias[4];
+  // the factors: tokens' in registers, channels' in shared memory.  Loads end
+  // in their order, so waiting for a stage waits for them too.
+  constexpr int EACH = (BN + THREADS - 1) / THREADS;
+  float sx[MT], sw[EACH], bias[EACH];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
     sx[i] = p.sx[b * p.M + min(m0 + (wm * MT + i) * 32 + row, p.M - 1)];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int64_t at = b * p.N + min(n + e, p.N - 1);
-    sw[e] = p.sw[at];
-    bias[e] = p.bias ? p.bias[at] : 0.f;
+  for (int i = 0; i < EACH; ++i) {
+    const int64_t at = b * p.N + min(n0 + i * THREADS + tid, p.N - 1);
+    sw[i] = p.sw[at];
+    bias[i] = p.bias ? p.bias[at] : 0.f;
   }
-  // these have arrived: from here on only stages are counted
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
   for (int s = 0; s < S - 1; ++s) fetch(s * BK, s);
+  float* factors = reinterpret_cast<float*>(shared + tiled_room(WN, WM, NT, MT, S));
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int c = i * THREADS + tid;
+    if (c < BN) {
+      factors[c] = sw[i];
+      factors[BN + c] = bias[i];
+    }
+  }
 
   v16i acc[NT][MT];
 #pragma unroll
@@ -671,146 +751,121 @@ __global__ __launch_bounds__(64 * WN * WM) void tiled_kernel(
       for (int e = 0; e < 16; ++e) acc[j][i][e] = 0;
 
   const int wrow = wn * NT * 32 + row, xrow = BN + wm * MT * 32 + row;
-  auto step = [&](const int8_t* stage, int left, auto masked) {
+  // the operands of step s of a stage (32 codes of K)
+  auto read = [&](const int8_t* stage, int s, v4i (&a)[NT], v4i (&x)[MT]) {
 #pragma unroll
-    for (int s = 0; s < BK / 32; ++s) {
-      v4i a[NT], x[MT];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const int r = wrow + 32 * j;
-        a[j] = *reinterpret_cast<const v4i*>(
-            stage + r * BK + (((2 * s + half) ^ place(r)) << 4));
-      }
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const int r = xrow + 32 * i;
-        x[i] = *reinterpret_cast<const v4i*>(
-            stage + r * BK + (((2 * s + half) ^ place(r)) << 4));
-      }
-      if constexpr (decltype(masked)::value) {  // tokens are 0 behind K
-        const int have_k = left - (2 * s + half) * 16;
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int c = have_k - 4 * j;
-            x[i][j] &= c >= 4 ? -1 : c <= 0 ? 0 : (1 << (8 * c)) - 1;
-          }
-      }
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-          acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[j], x[i],
-                                                            acc[j][i], 0, 0, 0);
+    for (int j = 0; j < NT; ++j) {
+      const int r = wrow + 32 * j;
+      a[j] = *reinterpret_cast<const v4i*>(
+          stage + r * BK + (((2 * s + half) ^ place(r)) << 4));
     }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int r = xrow + 32 * i;
+      x[i] = *reinterpret_cast<const v4i*>(
+          stage + r * BK + (((2 * s + half) ^ place(r)) << 4));
+    }
+  };
+  auto multiply = [&](const v4i (&a)[NT], const v4i (&x)[MT]) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+        acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[j], x[i], acc[j][i],
+                                                          0, 0, 0);
   };
 
   // A turn waits for its stage's own loads, then at the barrier for all waves':
   // by then they have also read the stage before it, whose place the next loads
   // take.  Loads behind the last stage repeat row begins, to keep the count.
+  // The first two steps' operands are asked for before the next stage is: 8192 x
+  // 4096 x 4096 148 -> 130 us.
   int turn = 0, k0 = 0;
   for (; k0 + BK <= p.K; k0 += BK) {
     wait_loads<PIECES * (S - 2)>();
     __builtin_amdgcn_s_barrier();
+    const int8_t* stage = shared + turn * STAGE;
+    v4i a[STEPS][NT], x[STEPS][MT];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) read(stage, s, a[s], x[s]);
     fetch(k0 + (S - 1) * BK, turn == 0 ? S - 1 : turn - 1);
-    step(shared + turn * STAGE, BK, std::false_type{});
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      if (s >= 2) read(stage, s, a[s], x[s]);
+      multiply(a[s], x[s]);
+    }
     turn = turn == S - 1 ? 0 : turn + 1;
   }
-  if (k0 < p.K) {
+  if (k0 < p.K) {  // the stage that K ends in
     wait_loads<PIECES * (S - 2)>();
     __builtin_amdgcn_s_barrier();
-    step(shared + turn * STAGE, p.K - k0, std::true_type{});
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      v4i a[NT], x[MT];
+      read(shared + turn * STAGE, s, a, x);
+      const int left = p.K - k0 - (2 * s + half) * 16;
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {  // tokens are 0 behind K
+          const int c = left - 4 * j;
+          x[i][j] &= c >= 4 ? -1 : c <= 0 ? 0 : (1 << (8 * c)) - 1;
+        }
+      multiply(a, x);
+    }
   }
   wait_loads<0>();
   __syncthreads();
 
   // 32 tokens x 32 NT channels at a time through the wave's own part of shared
-  // memory, to store whole rows
-  constexpr int ROW = NT * 32 + 4;
-  int* mine = reinterpret_cast<int*>(shared) + wave * 32 * ROW;
-#pragma unroll 1
-  for (int i = 0; i < MT; ++i) {
-    float sxi = sx[0];
-#pragma unroll
-    for (int ii = 0; ii < MT; ++ii) {
-      if (i != ii) continue;
-      sxi = sx[ii];
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const v4i sum = {acc[j][ii][4 * g], acc[j][ii][4 * g + 1],
-                           acc[j][ii][4 * g + 2], acc[j][ii][4 * g + 3]};
-          *reinterpret_cast<v4i*>(mine + row * ROW + j * 32 + 8 * g +
-                                  4 * half) = sum;
-        }
-    }
-    __builtin_amdgcn_wave_barrier();
-    auto rows = [&](auto count, int t0) {
-      constexpr int Q = decltype(count)::value;
-      v4f v[Q];
-      int m[Q];
-#pragma unroll
-      for (int q = 0; q < Q; ++q) {
-        const int t = t0 + q * TOKENS + lane / LANES;
-        m[q] = m0 + (wm * MT + i) * 32 + t;
-        const v4i sum = *reinterpret_cast<const v4i*>(mine + t * ROW +
-                                                      lane % LANES * 4);
-        const float s = __shfl(sxi, t);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          v[q][e] = finish(sum[e], s, sw[e], bias[e], Q == 1 ? p.act : p.act & 1);
-      }
-      put_rows<Q>(p, b, m, n, have, v);
-    };
-    if (p.act == 2) {
-#pragma unroll 1
-      for (int t0 = 0; t0 < 32; t0 += TOKENS)
-        rows(std::integral_constant<int, 1>{}, t0);
-    } else {
-#pragma unroll 1
-      for (int t0 = 0; t0 < 32; t0 += 4 * TOKENS)
-        rows(std::integral_constant<int, 4>{}, t0);
-    }
-    __builtin_amdgcn_wave_barrier();
-  }
+  // memory, to store 16 bytes of a token's row a lane
+  const int nw = wn * NT * 32, mw = m0 + wm * MT * 32;
+  int8_t* mine = shared + wave * tile_room(NT);
+  if (p.out != ELEM_F32 && p.act != 2)
+    tile_end<NT, MT, 8>(p, b, acc, sx, factors + nw, factors + BN + nw, mine,
+                        lane, n0 + nw, mw);
+  else
+    tile_end<NT, MT, 4>(p, b, acc, sx, factors + nw, factors + BN + nw, mine,
+                        lane, n0 + nw, mw);
 }
 
-template <int WN, int WM, int NT, int MT, int BK, int S>
-void launch_tiled(const DesInt8Product& p, hipStream_t stream) {
+template <int WN, int WM, int NT, int MT, int S>
+void launch_tiled(const DesInt8Product& p, bool together, hipStream_t stream) {
   constexpr int BN = 32 * WN * NT, BM = 32 * WM * MT;
-  constexpr int bytes = std::max(S * (BN + BM) * BK,
-                                 WN * WM * 32 * (NT * 32 + 4) * 4);
+  constexpr int bytes = tiled_room(WN, WM, NT, MT, S) + BN * 8;
   const uint32_t nblocks = (p.N + (int64_t)BN - 1) / BN;
   const uint32_t mblocks = (p.M + (int64_t)BM - 1) / BM;
-  auto kernel = tiled_kernel<WN, WM, NT, MT, BK, S>;
+  auto kernel = tiled_kernel<WN, WM, NT, MT, S>;
   if (bytes > 64 * 1024)
     (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                               hipFuncAttributeMaxDynamicSharedMemorySize,
                               bytes);
   hipLaunchKernelGGL(kernel, dim3((uint32_t)(p.B * nblocks * mblocks)),
-                     dim3(64 * WN * WM), bytes, stream, p, nblocks, mblocks);
+                     dim3(64 * WN * WM), bytes, stream, p, nblocks, mblocks,
+                     together);
 }
 
-// The largest tiles that give each of the chip's 256 units one, measured in us:
+// The largest tiles that still give each of the chip's 256 units one (two of
+// 128 x 128).  Neighbouring tiles are computed on one die, whose cache then
+// reads their tokens once; with 8 or more tiles in a row of 256 x 256 ones the
+// order as it comes does that for the weights.  us:
 //                        256 x 256  128 x 128  128 x 64  64 x 64
-//   8192 x 4096 x 4096       152        201       186      227
-//   8192 x  512 x 3136        52         25.0      25.8     36
-//   2048 x 2048 x 2048        37         18.7      17.7     20
-//   1024 x  512 x 3136        45         22        15.1     10.7
+//   8192 x 4096 x 4096       130        152       182      215
+//   8192 x  512 x 3136        46         33        23       36
+//   4096 x 1024 x 2048        30         17        15       19
+//   1024 x  512 x 3136        40         19        13        9
 void choose_tiled(const DesInt8Product& p, hipStream_t stream) {
   auto tiles = [&](int64_t n, int64_t m) {
     return p.B * ((p.N + n - 1) / n) * ((p.M + m - 1) / m);
   };
   if (tiles(256, 256) >= 256)
-    launch_tiled<2, 4, 4, 2, 128, 2>(p, stream);
-  else if (tiles(128, 128) >= 256)
-    launch_tiled<2, 2, 2, 2, 64, 3>(p, stream);
+    launch_tiled<2, 4, 4, 2, 2>(p, p.N <= 7 * 256, stream);
+  else if (tiles(128, 128) >= 512)
+    launch_tiled<2, 2, 2, 2, 2>(p, true, stream);
   else if (tiles(128, 64) >= 256)
-    launch_tiled<2, 2, 2, 1, 128, 2>(p, stream);
+    launch_tiled<2, 2, 2, 1, 2>(p, true, stream);
   else
-    launch_tiled<2, 2, 1, 1, 128, 3>(p, stream);
+    launch_tiled<2, 2, 1, 1, 3>(p, true, stream);
 }
 
 // codes -> rows every `step` bytes, with zeros behind them

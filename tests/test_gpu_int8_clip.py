@@ -154,6 +154,58 @@ def test_product_sizes(ops, m, n, k):
     _check_both(ops, x, wq, sw, bias, "none", torch.float32)
 
 
+@pytest.mark.parametrize("m,n,k", [
+    (4099, 4090, 300), (4096, 4096, 128), (8190, 2049, 77), (5, 900, 9000),
+    (4099, 2050, 515), (2048, 4096, 64), (16400, 250, 129), (16390, 64, 385),
+    (513, 4097, 256), (700, 1500, 1)])
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+def test_product_large_tiles(ops, m, n, k, out):
+    """Results enough for each size of tile, edges in both directions."""
+    x = _rand(m, k, seed=m + n + k)
+    wq, sw = _weights(ops, n, k)
+    bias = _rand(n, seed=2)
+    act = "tanh" if out == torch.float32 and k < 100 else "relu"
+    _check_both(ops, x, wq, sw, bias, act, out)
+
+
+def _sampled(ops, b, m, n, k, packed=False, seed=1):
+    """Many members, a few of them against 64 bits."""
+    step = k if packed else (k + 15) // 16 * 16
+    store = torch.randint(-127, 128, (b * n * step,), dtype=torch.int8,
+                          device="cuda",
+                          generator=torch.Generator("cuda").manual_seed(seed))
+    wq = store.view(b, n, step)[:, :, :k]
+    sw, bias = torch.rand(b, n, device="cuda") / 127, _rand(b, n, seed=3)
+    x = _rand(b, m, k, seed=4)
+    at = sorted({0, 1, b // 3, b // 2, b - 2, b - 1})
+    q, s = oracle.codes_and_scale(x[at])
+    want, err = oracle.product(q, s, wq[at], sw[at], bias[at], "none")
+    got = ops.int8_linear(x, wq, sw, bias)
+    oracle.check_product(got[at], want, err, torch.float32)
+    xq, sx = ops.quantize_rows(x)
+    assert torch.equal(ops.int8_matmul(xq, sx, wq, sw, bias), got)
+
+
+@pytest.mark.parametrize("m", [1, 3])
+@pytest.mark.parametrize("b,n,k,packed", [
+    (9000, 100, 376, False), (9000, 100, 375, True), (9000, 101, 384, False),
+    (900, 100, 3136, False), (900, 101, 3137, True), (900, 100, 3200, False),
+    (300, 70, 2000, False), (1000, 200, 250, True), (3000, 210, 60, False),
+    (9000, 300, 16, False), (9000, 300, 13, True), (20000, 110, 33, True)])
+def test_member_products_as_streams(ops, b, m, n, k, packed):
+    """Weights of 33 MB to 400 MB: every way of the stream of weights."""
+    _sampled(ops, b, m, n, k, packed)
+
+
+@pytest.mark.parametrize("b,m,n,k,packed", [
+    (1000, 16, 130, 376, False), (1000, 5, 130, 375, True),
+    (700, 20, 130, 376, False), (700, 31, 129, 375, True),
+    (100, 40, 129, 375, True), (60, 70, 300, 500, False),
+    (20, 300, 500, 129, True)])
+def test_member_products_of_more_tokens(ops, b, m, n, k, packed):
+    _sampled(ops, b, m, n, k, packed)
+
+
 @pytest.mark.parametrize("b,m,n,k", [
     (1, 1, 1, 1), (16, 1, 64, 64), (16, 1, 64, 4), (5, 1, 2, 64),
     (7, 1, 17, 256), (3, 1, 256, 376), (2, 2, 512, 3136), (3, 16, 33, 65),
@@ -179,7 +231,7 @@ def test_product_types_and_activations(ops, out, dtype, act, lead, m):
     _check_both(ops, x, wq, sw, None, act, out)
 
 
-@pytest.mark.parametrize("m", [1, 20, 200, 600])
+@pytest.mark.parametrize("m", [1, 20, 200, 600, 7000])
 def test_product_largest_sums(ops, m):
     """Codes of 127 throughout: 131072 * 127^2 is just inside 32 bits."""
     k = 131072
@@ -408,7 +460,8 @@ def _chain(ops, lead, m, seed):
     return x, layers, grads
 
 
-@pytest.mark.parametrize("lead,m", [((9,), 1), ((), 300)])
+@pytest.mark.parametrize("lead,m", [((9,), 1), ((), 16), ((), 300),
+                                    ((), 70000)])
 def test_captured_and_replayed(ops, lead, m):
     """Two graphs and eager calls in turn: each replay gives what an eager call
     on the inputs of that moment gives."""
