@@ -434,7 +434,7 @@ int64_t total_of(const std::vector<Tensor>& tensors) {
 
 // Few values in few tensors: one block does it all in one launch.
 bool is_small(const std::vector<Tensor>& tensors) {
-  return tensors.size() <= 32 && total_of(tensors) <= 1 << 15;
+  return tensors.size() <= DES_CLIP_TENSORS && total_of(tensors) <= 1 << 15;
 }
 
 // A share of a tensor is one block's work (a wave's, where it is small): 2^12

@@ -142,5 +142,5 @@ inline DesInt8Plan des_int8_plan(int64_t B, int64_t M, int64_t N, int64_t K) {
 // Whether int8_linear is one launch (every block quantises its tokens itself) or
 // two: a block's 1000 values take about 0.1 us, a launch of its own 2 to 4.
 inline bool des_int8_fused(int64_t M, int64_t K) {
-  return M <= 16 && M * K <= 16384;
+  return M <= 4 ? M * K <= 16384 : M <= 16 && K <= 512;
 }

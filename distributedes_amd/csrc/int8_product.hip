@@ -167,6 +167,65 @@ __device__ void quantize_block(const T* x, int64_t xsr, int rows, int K,
   __syncthreads();
 }
 
+// The same for rows of at most 64 NP values: 2^lbits lanes of a wave take a row,
+// up to NP pieces of 4 values each, which stay in registers, so that all rows
+// are read at once.  (16 rows of 40 values one after the other took 10 times
+// the product that they were for.)
+template <typename T, int NP>
+__device__ __forceinline__ void quantize_rows_at_once(
+    const T* x, int64_t xsr, int rows, int K, int kpad, int step,
+    int8_t* codes, float* scales, int lbits, int waves) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int L = 1 << lbits, per = 64 >> lbits;
+  const int k0 = (lane & (L - 1)) * 4;
+  for (int r0 = wave * per; r0 < rows; r0 += waves * per) {
+    const int r = r0 + (lane >> lbits);
+    const bool in = r < rows;
+    const T* src = x + (in ? r : 0) * xsr;
+    float v[NP][4];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+      load_floats(src, k0 + i * L * 4, in ? K : 0, v[i]);
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = max(top, abs_bits(v[i][j]));
+    for (int off = L >> 1; off > 0; off >>= 1)
+      top = max(top, (uint32_t)__shfl_xor((int)top, off));
+    const RowScale rs = row_scale(top);
+    if (!in) continue;
+    if (k0 == 0) scales[r] = rs.scale;
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+      if (k0 + i * L * 4 < kpad)
+        *reinterpret_cast<uint32_t*>(codes + r * step + k0 + i * L * 4) =
+            row_codes(v[i], rs);
+  }
+  __syncthreads();
+}
+
+// A block's float rows, by the one that fits.  `tops`: rows x waves words.
+template <typename T>
+__device__ __forceinline__ void quantize_tokens(const T* x, int64_t xsr,
+                                                int rows, int K, int kpad,
+                                                int step, int8_t* codes,
+                                                float* scales, uint32_t* tops,
+                                                int waves) {
+  // kpad may reach 64 values behind K: lanes for all of it
+  int lbits = 0;
+  if (kpad <= 1024) {
+    while ((16 << lbits) < kpad) ++lbits;
+    quantize_rows_at_once<T, 4>(x, xsr, rows, K, kpad, step, codes, scales,
+                                lbits, waves);
+  } else if (kpad <= 2048) {
+    quantize_rows_at_once<T, 8>(x, xsr, rows, K, kpad, step, codes, scales, 6,
+                                waves);
+  } else {
+    quantize_block(x, xsr, rows, K, kpad, step, codes, scales, tops, waves);
+  }
+}
+
 // Copies rows of K codes into shared memory, a row every `step` bytes with
 // zeros up to `kpad` (a multiple of 16).
 __device__ void stage_block(const int8_t* x, int64_t xsr, int rows, int K,
@@ -235,8 +294,12 @@ __global__ __launch_bounds__(256) void gemv_kernel(DesInt8Product p, int lbits,
 
   if constexpr (FLOATS) {
     uint32_t* tops = reinterpret_cast<uint32_t*>(sums + waves * 64 * MR);
-    quantize_block((const X*)p.xf + b * p.xsb, p.xsr, p.M, p.K, kpad, step,
-                   codes, scales, tops, waves);
+    const X* xf = (const X*)p.xf + b * p.xsb;
+    if constexpr (MR == 1)  // one row: all waves, and fewer registers
+      quantize_block(xf, p.xsr, 1, p.K, kpad, step, codes, scales, tops, waves);
+    else
+      quantize_tokens(xf, p.xsr, p.M, p.K, kpad, step, codes, scales, tops,
+                      waves);
   } else {
     stage_block(p.x + b * p.xsb, p.xsr, p.M, p.K, kpad, step, codes, p.xwhole);
   }
@@ -395,8 +458,8 @@ __global__ __launch_bounds__(1024) void stream_kernel(DesInt8Product p, int wn,
     const int rows = min(16, p.M - m0);
     const X* xf = (const X*)p.xf + b * p.xsb + m0 * p.xsr;
     uint32_t* tops = reinterpret_cast<uint32_t*>(codes + rows * xstep);
-    quantize_block(xf, p.xsr, rows, p.K, steps * 64, xstep, codes, scales, tops,
-                   waves);
+    quantize_tokens(xf, p.xsr, rows, p.K, steps * 64, xstep, codes, scales,
+                    tops, waves);
   }
   const int8_t* wr[NT];
   const int8_t* xr[MT];
