@@ -21,10 +21,10 @@
 #include "int8.h"
 
 extern "C" {
-void des_launch_quantize_rows(const void*, int, int64_t, int64_t, int8_t*,
+bool des_launch_quantize_rows(const void*, int, int64_t, int64_t, int8_t*,
                               int64_t, int64_t, float*, int64_t, int64_t, int,
                               hipStream_t);
-void des_launch_int8_product(const DesInt8Product*, hipStream_t);
+bool des_launch_int8_product(const DesInt8Product*, hipStream_t);
 void des_launch_pack_rows(const int8_t*, int64_t, int64_t, int8_t*, int64_t,
                           int64_t, int, hipStream_t);
 void des_launch_square_sums(const DesClipTable*, int64_t, double*,
@@ -43,6 +43,7 @@ using c10::optional;
 
 constexpr int64_t MAX_COLS = 131072;  // int32 sums of 127 * 127 stay in range
 constexpr int64_t MAX_INT = 2147483647;
+constexpr int64_t MAX_ROWS = 1 << 30;  // of a product: 32 bits hold a tile more
 
 inline hipStream_t cur_stream() {
   return at::hip::getCurrentHIPStream().stream();
@@ -165,11 +166,13 @@ void launch_quantize(const Tensor& x, const Tensor& q, const Tensor& s) {
       qr = Rows{xr.lead, xr.rows, xr.rows * qr.sr, qr.sr};
     }
   }
-  TORCH_CHECK_VALUE(rows <= MAX_INT, "too many rows: ", rows);
-  des_launch_quantize_rows(x.data_ptr(), elem_of(x.scalar_type(), "x"), xr.sl,
-                           xr.sr, q.data_ptr<int8_t>(), qr.sl, qr.sr,
-                           s.data_ptr<float>(), xr.lead, xr.rows, (int)cols,
-                           cur_stream());
+  TORCH_CHECK_VALUE(
+      rows <= MAX_INT &&
+          des_launch_quantize_rows(
+              x.data_ptr(), elem_of(x.scalar_type(), "x"), xr.sl, xr.sr,
+              q.data_ptr<int8_t>(), qr.sl, qr.sr, s.data_ptr<float>(), xr.lead,
+              xr.rows, (int)cols, cur_stream()),
+      rows, " rows are too many for one call");
   CHECK_LAUNCH();
 }
 
@@ -321,13 +324,13 @@ Tensor product(const Tensor& x_, const Tensor& sx_, const Tensor& wq_,
     as_rows(x, &r);
     if (r.lead != 1) x = x.contiguous();
     as_rows(x, &r);
-    TORCH_CHECK_VALUE(r.rows <= MAX_INT, "too many rows: ", r.rows);
+    TORCH_CHECK_VALUE(r.rows <= MAX_ROWS, "too many rows: ", r.rows);
     p.B = 1;
     p.M = (int32_t)r.rows;
     p.xsb = 0;
     p.xsr = r.sr;
   } else {
-    TORCH_CHECK_VALUE(x.size(1) <= MAX_INT, "too many rows: ", x.size(1));
+    TORCH_CHECK_VALUE(x.size(1) <= MAX_ROWS, "too many rows: ", x.size(1));
     p.B = x.size(0);
     p.M = (int32_t)x.size(1);
     p.xsb = x.stride(0);
@@ -355,7 +358,7 @@ Tensor product(const Tensor& x_, const Tensor& sx_, const Tensor& wq_,
   }
   const Tensor wq =
       K > 1 && wq_.stride(-1) != 1 ? wq_.contiguous() : wq_;
-  TORCH_CHECK_VALUE(wq.size(-2) <= MAX_INT, "too many channels");
+  TORCH_CHECK_VALUE(wq.size(-2) <= MAX_ROWS, "too many channels");
   p.N = (int32_t)wq.size(-2);
   p.K = (int32_t)K;
   p.wsb = members ? wq.stride(0) : 0;
@@ -369,15 +372,14 @@ Tensor product(const Tensor& x_, const Tensor& sx_, const Tensor& wq_,
   p.y = y.data_ptr();
   p.act = act;
   p.out = elem_of(out_dtype, "out_dtype");
-  const double tiles = (double)p.B * ((p.M + 15) / 16) * ((p.N + 15) / 16);
-  TORCH_CHECK_VALUE(tiles <= (double)MAX_INT, "a product of ", p.B, " x ", p.M,
-                    " x ", p.N, " results is too large for one call");
   Tensor x_copy, w_copy;
   if (K > 0 && des_int8_plan(p.B, p.M, p.N, p.K) == DES_INT8_TILED) {
     p.x = aligned_rows(p.x, &p.xsb, &p.xsr, p.B, p.M, K, p.xwhole, y, &x_copy);
     p.w = aligned_rows(p.w, &p.wsb, &p.wsr, p.B, p.N, K, p.wwhole, y, &w_copy);
   }
-  des_launch_int8_product(&p, cur_stream());
+  TORCH_CHECK_VALUE(des_launch_int8_product(&p, cur_stream()), "a product of ",
+                    p.B, " x ", p.M, " x ", p.N,
+                    " results is too large for one call");
   CHECK_LAUNCH();
   return y;
 }

@@ -368,17 +368,32 @@ __global__ __launch_bounds__(256) void gemv_kernel(DesInt8Product p, int lbits,
   }
 }
 
+// waves of a block for parts of a member's channels: up to 4, and as even as the
+// blocks that this takes allow (5 parts: 3 + 2, not 4 + 1)
+int waves_for(int64_t parts) {
+  const int64_t blocks = (parts + 3) / 4;
+  return (int)((parts + blocks - 1) / blocks);
+}
+
+// A launch has at most 2^31 - 1 blocks and 2^32 - 1 threads; a larger one is not
+// begun.
+bool fits(int64_t blocks, int threads) {
+  return blocks <= 0x7FFFFFFF && blocks * threads <= 0xFFFFFFFF;
+}
+
 template <typename X, int MR, int U, bool ONCE>
-void launch_gemv(const DesInt8Product& p, int lbits, int rows_a_wave,
+bool launch_gemv(const DesInt8Product& p, int lbits, int rows_a_wave,
                  hipStream_t stream) {
   const int64_t parts = (p.N + (int64_t)rows_a_wave - 1) / rows_a_wave;
-  const int waves = (int)std::min<int64_t>(4, parts);
+  const int waves = waves_for(parts);
   const int64_t nblocks = (parts + waves - 1) / waves;
   const size_t bytes = 16 + p.M * ((p.K + 15) / 16 * 16 + 16) +
                        waves * 64 * MR * 4 + p.M * waves * 4;
+  if (!fits(p.B * nblocks, 64 * waves)) return false;
   hipLaunchKernelGGL((gemv_kernel<X, MR, U, ONCE>),
                      dim3((uint32_t)(p.B * nblocks)), dim3(64 * waves), bytes,
                      stream, p, lbits, rows_a_wave);
+  return true;
 }
 
 // How many lanes take a row, how many rows a wave takes, and whether its loads
@@ -394,7 +409,7 @@ void launch_gemv(const DesInt8Product& p, int lbits, int rows_a_wave,
 //    which have fewer sums to join.  K = 200 (208): 2 lanes 255 us, 4 130, 8 104,
 //    16 99; past the caches 150.  K = 48: 1 lane 139, 2 124, 4 138.
 template <typename X, int MR>
-void choose_gemv_rows(const DesInt8Product& p, hipStream_t stream) {
+bool choose_gemv_rows(const DesInt8Product& p, hipStream_t stream) {
   const int64_t bytes = p.B * (int64_t)p.N * p.K;
   auto lanes = [&](int codes, int least, int most) {  // as bits
     int bits = least;
@@ -403,28 +418,24 @@ void choose_gemv_rows(const DesInt8Product& p, hipStream_t stream) {
   };
   if (bytes <= 32 << 20) {
     const int bits = lanes(16, 0, 6);
-    launch_gemv<X, MR, 1, false>(p, bits, 64 >> bits, stream);
-    return;
+    return launch_gemv<X, MR, 1, false>(p, bits, 64 >> bits, stream);
   }
   const int rows = p.K >= 1024 ? 16 : 64;
   const bool lines =
       ((uintptr_t)p.w | (uintptr_t)p.wsr | (uintptr_t)p.wsb) % 128 == 0;
   const bool once = bytes >= 256 << 20;
   if (once && lines && p.K > 96)
-    launch_gemv<X, MR, 2, true>(p, 3, rows, stream);
-  else if (once && p.K >= 2048)
-    launch_gemv<X, MR, 4, true>(p, 6, rows, stream);
-  else
-    launch_gemv<X, MR, 2, false>(p, p.K <= 16 ? 0 : lanes(32, 1, 4), rows,
-                                 stream);
+    return launch_gemv<X, MR, 2, true>(p, 3, rows, stream);
+  if (once && p.K >= 2048)
+    return launch_gemv<X, MR, 4, true>(p, 6, rows, stream);
+  return launch_gemv<X, MR, 2, false>(p, p.K <= 16 ? 0 : lanes(32, 1, 4), rows,
+                                      stream);
 }
 
 template <typename X>
-void choose_gemv(const DesInt8Product& p, hipStream_t stream) {
-  if (p.M == 1)
-    choose_gemv_rows<X, 1>(p, stream);
-  else
-    choose_gemv_rows<X, 4>(p, stream);
+bool choose_gemv(const DesInt8Product& p, hipStream_t stream) {
+  return p.M == 1 ? choose_gemv_rows<X, 1>(p, stream)
+                  : choose_gemv_rows<X, 4>(p, stream);
 }
 
 // Few rows: weights go straight from memory into the matrix instruction's
@@ -482,7 +493,7 @@ __global__ __launch_bounds__(1024) void stream_kernel(DesInt8Product p, int wn,
 
   const int share = wave / wn;
   const int s0 = (int)((int64_t)steps * share / wk);
-  const int s1 = (int)((int64_t)steps * (share + 1) / wk);
+  const int s1 = n0 < p.N ? (int)((int64_t)steps * (share + 1) / wk) : s0;
   const int s1f = min(s1, full);
 #pragma unroll 4
   for (int s = s0; s < s1f; ++s) {
@@ -551,7 +562,7 @@ __global__ __launch_bounds__(1024) void stream_kernel(DesInt8Product p, int wn,
 }
 
 template <typename X, int MT, int NT>
-void launch_stream(const DesInt8Product& p, int wn, int wk,
+bool launch_stream(const DesInt8Product& p, int wn, int wk,
                    hipStream_t stream) {
   const int64_t nblocks = (p.N + 16 * NT * wn - 1) / (16 * NT * wn);
   const int64_t mblocks = (p.M + 16 * MT - 1) / (16 * MT);
@@ -560,9 +571,11 @@ void launch_stream(const DesInt8Product& p, int wn, int wk,
   if (sizeof(X) != 1)
     bytes += rows * ((p.K + 63) / 64 * 64 + 16) + rows * waves * 4;
   bytes = std::max<size_t>(bytes, 64 + (size_t)(wk - 1) * wn * MT * NT * 1024);
+  if (!fits(p.B * nblocks * mblocks, 64 * waves)) return false;
   hipLaunchKernelGGL((stream_kernel<X, MT, NT>),
                      dim3((uint32_t)(p.B * nblocks * mblocks)),
                      dim3(64 * waves), bytes, stream, p, wn, wk);
+  return true;
 }
 
 // Many members fill the chip with waves of 64 channels (or, for 17 to 32
@@ -570,34 +583,28 @@ void launch_stream(const DesInt8Product& p, int wn, int wk,
 // K.  For one policy of 512 x 3136: 16 to 128 tokens 5.2 us, in groups of 16
 // tokens; 256 tokens in groups of 32 6.8; 512 tokens in groups of 32 x 32 8.7.
 template <typename X>
-void choose_stream(const DesInt8Product& p, hipStream_t stream) {
+bool choose_stream(const DesInt8Product& p, hipStream_t stream) {
   const int64_t groups = (p.N + 15) / 16, steps = (p.K + 63) / 64;
   const int64_t blocks = p.B * ((p.M + 15) / 16) * groups;
   if (p.M <= 16 && blocks >= 4 * 2048 && groups >= 4) {
-    launch_stream<X, 1, 4>(p, (int)std::min<int64_t>(4, (groups + 3) / 4), 1,
-                           stream);
-    return;
+    return launch_stream<X, 1, 4>(p, waves_for((groups + 3) / 4), 1, stream);
   }
   if constexpr (sizeof(X) == 1) {
     if (p.M > 16 && p.B > 1 && blocks >= 4096) {
-      launch_stream<X, 2, 2>(p, (int)std::min<int64_t>(4, (groups + 1) / 2), 1,
-                             stream);
-      return;
+      return launch_stream<X, 2, 2>(p, waves_for((groups + 1) / 2), 1, stream);
     }
     if (blocks > 1024) {
-      launch_stream<X, 2, 2>(p, 1, steps >= 4 ? 4 : 1, stream);
-      return;
+      return launch_stream<X, 2, 2>(p, 1, steps >= 4 ? 4 : 1, stream);
     }
     if (blocks > 256 && p.M > 16) {
-      launch_stream<X, 2, 1>(p, 1, steps >= 8 ? 8 : steps >= 4 ? 4 : 1, stream);
-      return;
+      return launch_stream<X, 2, 1>(p, 1, steps >= 8 ? 8 : steps >= 4 ? 4 : 1, stream);
     }
   }
   int wn = 1, wk = 1;
   while (wk < 8 && blocks * wk < 2048 && steps >= 2 * wk) wk *= 2;
   if (wk == 8 && blocks <= 64 && steps >= 32) wk = 16;
   while (wn * wk < 4 && wn < groups) wn *= 2;
-  launch_stream<X, 1, 1>(p, wn, wk, stream);
+  return launch_stream<X, 1, 1>(p, wn, wk, stream);
 }
 
 typedef __attribute__((ext_vector_type(16))) int v16i;
@@ -610,11 +617,20 @@ __device__ __forceinline__ void load_shared(const int8_t* from, int8_t* to) {
       (__attribute__((address_space(3))) void*)to, 16, 0, 0);
 }
 
-// until at most N loads are under way
+// Until at most N of this wave's loads are under way and its reads of shared
+// memory have ended, then until all waves are here.  One statement, which no
+// access to memory is moved across.
 template <int N>
-__device__ __forceinline__ void wait_loads() {
-  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) |
-                             ((N >> 4) << 14));
+__device__ __forceinline__ void wait_stage() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N)
+               : "memory");
+}
+
+// Between writes and reads of shared memory by lanes of one wave, which the
+// hardware takes in their order: the compiler has to keep it too.
+__device__ __forceinline__ void wave_order() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_wave_barrier();
 }
 
 // a wave's shared memory for 32 tokens x 32 NT results of 4 bytes
@@ -674,7 +690,7 @@ __device__ __forceinline__ void tile_end(const DesInt8Product& p, int64_t b,
           }
         }
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_order();
     const int8_t* from = mine + lane / LANES * ROW + lane % LANES * 16;
     int m = m0 + i * 32 + lane / LANES;
     int64_t at = (b * p.M + m) * p.N + n;
@@ -711,7 +727,7 @@ __device__ __forceinline__ void tile_end(const DesInt8Product& p, int64_t b,
       m += TOKENS;
       at += (int64_t)TOKENS * p.N;
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_order();
   }
 }
 
@@ -845,8 +861,7 @@ __global__ __launch_bounds__(64 * WN * WM) void tiled_kernel(
   // 4096 x 4096 148 -> 130 us.
   int turn = 0, k0 = 0;
   for (; k0 + BK <= p.K; k0 += BK) {
-    wait_loads<PIECES * (S - 2)>();
-    __builtin_amdgcn_s_barrier();
+    wait_stage<PIECES * (S - 2)>();
     const int8_t* stage = shared + turn * STAGE;
     v4i a[STEPS][NT], x[STEPS][MT];
 #pragma unroll
@@ -860,8 +875,7 @@ __global__ __launch_bounds__(64 * WN * WM) void tiled_kernel(
     turn = turn == S - 1 ? 0 : turn + 1;
   }
   if (k0 < p.K) {  // the stage that K ends in
-    wait_loads<PIECES * (S - 2)>();
-    __builtin_amdgcn_s_barrier();
+    wait_stage<PIECES * (S - 2)>();
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
       v4i a[NT], x[MT];
@@ -877,8 +891,7 @@ __global__ __launch_bounds__(64 * WN * WM) void tiled_kernel(
       multiply(a, x);
     }
   }
-  wait_loads<0>();
-  __syncthreads();
+  wait_stage<0>();  // the loads behind K as well: their room is used again
 
   // 32 tokens x 32 NT channels at a time through the wave's own part of shared
   // memory, to store 16 bytes of a token's row a lane
@@ -893,19 +906,21 @@ __global__ __launch_bounds__(64 * WN * WM) void tiled_kernel(
 }
 
 template <int WN, int WM, int NT, int MT, int S>
-void launch_tiled(const DesInt8Product& p, bool together, hipStream_t stream) {
+bool launch_tiled(const DesInt8Product& p, bool together, hipStream_t stream) {
   constexpr int BN = 32 * WN * NT, BM = 32 * WM * MT;
   constexpr int bytes = tiled_room(WN, WM, NT, MT, S) + BN * 8;
   const uint32_t nblocks = (p.N + (int64_t)BN - 1) / BN;
   const uint32_t mblocks = (p.M + (int64_t)BM - 1) / BM;
+  const int64_t blocks = p.B * (int64_t)nblocks * mblocks;
+  if (!fits(blocks, 64 * WN * WM)) return false;
   auto kernel = tiled_kernel<WN, WM, NT, MT, S>;
   if (bytes > 64 * 1024)
     (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                               hipFuncAttributeMaxDynamicSharedMemorySize,
                               bytes);
-  hipLaunchKernelGGL(kernel, dim3((uint32_t)(p.B * nblocks * mblocks)),
-                     dim3(64 * WN * WM), bytes, stream, p, nblocks, mblocks,
-                     together);
+  hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(64 * WN * WM), bytes,
+                     stream, p, nblocks, mblocks, together);
+  return true;
 }
 
 // The largest tiles that still give each of the chip's 256 units one (two of
@@ -917,18 +932,17 @@ void launch_tiled(const DesInt8Product& p, bool together, hipStream_t stream) {
 //   8192 x  512 x 3136        46         33        23       36
 //   4096 x 1024 x 2048        30         17        15       19
 //   1024 x  512 x 3136        40         19        13        9
-void choose_tiled(const DesInt8Product& p, hipStream_t stream) {
+bool choose_tiled(const DesInt8Product& p, hipStream_t stream) {
   auto tiles = [&](int64_t n, int64_t m) {
     return p.B * ((p.N + n - 1) / n) * ((p.M + m - 1) / m);
   };
   if (tiles(256, 256) >= 256)
-    launch_tiled<2, 4, 4, 2, 2>(p, p.N <= 7 * 256, stream);
-  else if (tiles(128, 128) >= 512)
-    launch_tiled<2, 2, 2, 2, 2>(p, true, stream);
-  else if (tiles(128, 64) >= 256)
-    launch_tiled<2, 2, 2, 1, 2>(p, true, stream);
-  else
-    launch_tiled<2, 2, 1, 1, 3>(p, true, stream);
+    return launch_tiled<2, 4, 4, 2, 2>(p, p.N <= 7 * 256, stream);
+  if (tiles(128, 128) >= 512)
+    return launch_tiled<2, 2, 2, 2, 2>(p, true, stream);
+  if (tiles(128, 64) >= 256)
+    return launch_tiled<2, 2, 2, 1, 2>(p, true, stream);
+  return launch_tiled<2, 2, 1, 1, 3>(p, true, stream);
 }
 
 // codes -> rows every `step` bytes, with zeros behind them
@@ -960,23 +974,21 @@ extern "C" void des_launch_pack_rows(const int8_t* from, int64_t sb, int64_t sr,
                      pieces);
 }
 
-extern "C" void des_launch_int8_product(const DesInt8Product* p,
+extern "C" bool des_launch_int8_product(const DesInt8Product* p,
                                         hipStream_t stream) {
   const DesInt8Product& q = *p;
   const DesInt8Plan plan = des_int8_plan(q.B, q.M, q.N, q.K);
-  if (plan == DES_INT8_TILED) {
-    choose_tiled(q, stream);
-  } else if (q.x) {
-    plan == DES_INT8_GEMV ? choose_gemv<int8_t>(q, stream)
-                          : choose_stream<int8_t>(q, stream);
-  } else if (q.xelem == ELEM_F32) {
-    plan == DES_INT8_GEMV ? choose_gemv<float>(q, stream)
-                          : choose_stream<float>(q, stream);
-  } else if (q.xelem == ELEM_BF16) {
-    plan == DES_INT8_GEMV ? choose_gemv<Bf16>(q, stream)
-                          : choose_stream<Bf16>(q, stream);
-  } else {
-    plan == DES_INT8_GEMV ? choose_gemv<_Float16>(q, stream)
-                          : choose_stream<_Float16>(q, stream);
-  }
+  if (plan == DES_INT8_TILED) return choose_tiled(q, stream);
+  const bool gemv = plan == DES_INT8_GEMV;
+  if (q.x)
+    return gemv ? choose_gemv<int8_t>(q, stream)
+                : choose_stream<int8_t>(q, stream);
+  if (q.xelem == ELEM_F32)
+    return gemv ? choose_gemv<float>(q, stream)
+                : choose_stream<float>(q, stream);
+  if (q.xelem == ELEM_BF16)
+    return gemv ? choose_gemv<Bf16>(q, stream)
+                : choose_stream<Bf16>(q, stream);
+  return gemv ? choose_gemv<_Float16>(q, stream)
+              : choose_stream<_Float16>(q, stream);
 }

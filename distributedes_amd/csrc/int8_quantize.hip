@@ -137,11 +137,28 @@ __global__ __launch_bounds__(1024) void block_rows_kernel(Rows p) {
   if (tid == 0) p.scale[blockIdx.x] = rs.scale;
 }
 
+// A launch has at most 2^32 - 1 threads; a larger one is not begun.
+bool fits(int64_t blocks, int threads) {
+  return blocks * threads <= 0xFFFFFFFF;
+}
+
 template <typename T, int R>
-void launch_waves(const Rows& p, int lbits, hipStream_t stream) {
+bool launch_waves(const Rows& p, int lbits, hipStream_t stream) {
   const uint32_t rows = p.lead * p.rows, per = 4u << (6 - lbits);
+  if (!fits((rows + per - 1) / per, 256)) return false;
   hipLaunchKernelGGL((wave_rows_kernel<T, R>), dim3((rows + per - 1) / per),
                      dim3(256), 0, stream, p, lbits);
+  return true;
+}
+
+template <typename T, int R>
+bool launch_blocks(const Rows& p, int64_t threads, hipStream_t stream) {
+  const uint32_t rows = p.lead * p.rows;
+  const int each = (int)std::min<int64_t>(1024, (threads + 63) / 64 * 64);
+  if (!fits(rows, each)) return false;
+  hipLaunchKernelGGL((block_rows_kernel<T, R>), dim3(rows), dim3(each), 0,
+                     stream, p);
+  return true;
 }
 
 // Pieces of 16 bytes and who takes them; measured:
@@ -153,41 +170,30 @@ void launch_waves(const Rows& p, int lbits, hipStream_t stream) {
 //  - few rows: a block, a piece a thread, for latency. 16 x 3136 bf16 by 448
 //    threads 4.2 us, 256 6.1.
 template <typename T>
-void choose(const Rows& p, hipStream_t stream) {
+bool choose(const Rows& p, hipStream_t stream) {
   constexpr int V = 16 / sizeof(T);
   const int64_t pieces = ((int64_t)p.cols + V - 1) / V;
   const uint32_t rows = p.lead * p.rows;
-  auto threads = [](int64_t n) {
-    return dim3((uint32_t)std::min<int64_t>(1024, (n + 63) / 64 * 64));
-  };
-  if (pieces > 64 && rows < 512) {
-    hipLaunchKernelGGL((block_rows_kernel<T, 1>), dim3(rows), threads(pieces),
-                       0, stream, p);
-    return;
-  }
-  if (pieces > 256) {
-    hipLaunchKernelGGL((block_rows_kernel<T, 4>), dim3(rows),
-                       threads((pieces + 3) / 4), 0, stream, p);
-    return;
-  }
+  if (pieces > 64 && rows < 512) return launch_blocks<T, 1>(p, pieces, stream);
+  if (pieces > 256) return launch_blocks<T, 4>(p, (pieces + 3) / 4, stream);
   int lbits = 0;
   while (lbits < 6 && (4 << lbits) < pieces) ++lbits;
   const int64_t turns = (pieces + (1 << lbits) - 1) >> lbits;
-  if (turns <= 1) launch_waves<T, 1>(p, lbits, stream);
-  else if (turns <= 2) launch_waves<T, 2>(p, lbits, stream);
-  else launch_waves<T, 4>(p, lbits, stream);
+  if (turns <= 1) return launch_waves<T, 1>(p, lbits, stream);
+  if (turns <= 2) return launch_waves<T, 2>(p, lbits, stream);
+  return launch_waves<T, 4>(p, lbits, stream);
 }
 
 }  // namespace
 
-extern "C" void des_launch_quantize_rows(const void* x, int elem, int64_t xsl,
+extern "C" bool des_launch_quantize_rows(const void* x, int elem, int64_t xsl,
                                          int64_t xsr, int8_t* q, int64_t qsl,
                                          int64_t qsr, float* scale,
                                          int64_t lead, int64_t rows, int cols,
                                          hipStream_t stream) {
   const Rows p = {x,   q,   scale,          xsl,            xsr,
                   qsl, qsr, (uint32_t)lead, (uint32_t)rows, cols};
-  if (elem == ELEM_F32) choose<float>(p, stream);
-  else if (elem == ELEM_BF16) choose<Bf16>(p, stream);
-  else choose<_Float16>(p, stream);
+  return elem == ELEM_F32    ? choose<float>(p, stream)
+         : elem == ELEM_BF16 ? choose<Bf16>(p, stream)
+                             : choose<_Float16>(p, stream);
 }
