@@ -134,13 +134,18 @@ std::vector<int64_t> lead_shape(const Tensor& x) {
 }
 
 // codes for rows of x's shape: rows begin at multiples of 16 bytes, which the
-// products' wide loads like
+// products' wide loads like, and the last row's gap belongs to the storage
 Tensor new_codes(const Tensor& x) {
-  auto shape = x.sizes().vec();
-  const int64_t cols = shape.back();
-  shape.back() = (cols + 15) / 16 * 16;
-  return at::empty(shape, x.options().dtype(at::kChar))
-      .narrow(-1, 0, cols);
+  const auto shape = x.sizes();
+  std::vector<int64_t> strides(shape.size(), 1);
+  int64_t total = (shape.back() + 15) / 16 * 16;
+  for (int64_t d = (int64_t)shape.size() - 2; d >= 0; --d) {
+    strides[d] = total;
+    total *= std::max<int64_t>(1, shape[d]);
+  }
+  Tensor q = at::empty({total}, x.options().dtype(at::kChar));
+  q.unsafeGetTensorImpl()->set_sizes_and_strides(shape, strides);
+  return q;
 }
 
 void check_float_rows(const Tensor& x) {
