@@ -133,12 +133,19 @@ std::vector<int64_t> lead_shape(const Tensor& x) {
   return {x.sizes().begin(), x.sizes().end() - 1};
 }
 
-// codes for rows of x's shape: rows begin at multiples of 16 bytes, which the
-// products' wide loads like, and the last row's gap belongs to the storage
+// Bytes from row to row of fresh codes: whole pieces of 16, which the products'
+// wide loads like, or whole lines of 128, where that adds 1/16 at most (a product
+// of 8192 x 512 x 3136 21.8 us instead of 23.9, with rows of 3200).
+int64_t row_step(int64_t cols) {
+  const int64_t line = (cols + 127) / 128 * 128;
+  return line - cols <= cols / 16 ? line : (cols + 15) / 16 * 16;
+}
+
+// codes for rows of x's shape; the last row's gap belongs to the storage
 Tensor new_codes(const Tensor& x) {
   const auto shape = x.sizes();
   std::vector<int64_t> strides(shape.size(), 1);
-  int64_t total = (shape.back() + 15) / 16 * 16;
+  int64_t total = row_step(shape.back());
   for (int64_t d = (int64_t)shape.size() - 2; d >= 0; --d) {
     strides[d] = total;
     total *= std::max<int64_t>(1, shape[d]);
@@ -350,7 +357,7 @@ Tensor product(const Tensor& x_, const Tensor& sx_, const Tensor& wq_,
     sx = at::empty(lead_shape(x), x.options().dtype(at::kFloat));
     launch_quantize(x, q, sx);
     x = q;
-    p.xsr = members ? q.stride(1) : (K + 15) / 16 * 16;
+    p.xsr = members ? q.stride(1) : row_step(K);
     p.xsb = members ? q.stride(0) : 0;
   }
   if (sx.defined()) {
@@ -516,7 +523,8 @@ Tensor global_norm(const std::vector<Tensor>& tensors) {
   return norm;
 }
 
-std::pair<std::vector<Tensor>, Tensor> clip_by_global_norm(
+// -> (the clipped tensors, or None where they are `out`; the norm)
+std::pair<optional<std::vector<Tensor>>, Tensor> clip_by_global_norm(
     const std::vector<Tensor>& tensors, double max_norm,
     const optional<std::vector<Tensor>>& out) {
   check_tensors(tensors);
@@ -559,6 +567,10 @@ std::pair<std::vector<Tensor>, Tensor> clip_by_global_norm(
   check_gpu(tensors[0]);
   const c10::DeviceGuard guard(tensors[0].device());
   std::vector<Tensor> in, to;
+  auto result = [&]() -> optional<std::vector<Tensor>> {
+    if (out.has_value()) return c10::nullopt;
+    return to;
+  };
   for (size_t i = 0; i < tensors.size(); ++i) {
     in.push_back(tensors[i].contiguous());
     to.push_back(out.has_value() ? (*out)[i] : at::empty_like(in[i]));
@@ -570,7 +582,7 @@ std::pair<std::vector<Tensor>, Tensor> clip_by_global_norm(
     des_launch_clip_small(&tables.tables[0], share, max_norm,
                           norm.data_ptr<float>(), true, cur_stream());
     CHECK_LAUNCH();
-    return {to, norm};
+    return {result(), norm};
   }
   const Tensor sums = square_sums(tables, share, in[0]);
   bool first = true;
@@ -584,7 +596,7 @@ std::pair<std::vector<Tensor>, Tensor> clip_by_global_norm(
     CHECK_LAUNCH();
     first = false;
   }
-  return {to, norm};
+  return {result(), norm};
 }
 
 }  // namespace

@@ -399,7 +399,7 @@ bool launch_gemv(const DesInt8Product& p, int lbits, int rows_a_wave,
 // How many lanes take a row, how many rows a wave takes, and whether its loads
 // pass the caches by.  Measured over 0.5 to 1 GB of weights, M = 1:
 //  - up to 32 MB: latency counts.  A row to as many lanes as it fills, one load
-//    a row and turn, and as many waves as that gives.
+//    a row and turn, and as many waves as that gives, up to 8192.
 //  - weights that no cache would keep (256 MB), rows that begin on lines of
 //    128 bytes: past the caches, a line a turn and row.  K = 376 (rows of 384):
 //    4 lanes 292 us, 8 163, 16 167, 32 192; through the caches 180.
@@ -418,7 +418,9 @@ bool choose_gemv_rows(const DesInt8Product& p, hipStream_t stream) {
   };
   if (bytes <= 32 << 20) {
     const int bits = lanes(16, 0, 6);
-    return launch_gemv<X, MR, 1, false>(p, bits, 64 >> bits, stream);
+    int rows = 64 >> bits;
+    while (rows < 64 && p.B * ((p.N + rows - 1) / rows) > 8192) rows *= 2;
+    return launch_gemv<X, MR, 1, false>(p, bits, rows, stream);
   }
   const int rows = p.K >= 1024 ? 16 : 64;
   const bool lines =
@@ -763,7 +765,7 @@ __global__ __launch_bounds__(64 * WN * WM) void tiled_kernel(
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wn = wave % WN, wm = wave / WN;
   uint32_t id = blockIdx.x;
-  if (together) {  // blocks in turn go to 8 dies: each takes a piece of the list
+  if (together) {  // each die takes a piece of the list (see tiles_together)
     const uint32_t each = gridDim.x / 8;
     if (id < 8 * each) id = (id & 7) * each + (id >> 3);
   }
@@ -905,8 +907,24 @@ __global__ __launch_bounds__(64 * WN * WM) void tiled_kernel(
                         lane, n0 + nw, mw);
 }
 
+// Whether neighbouring tiles are computed on one die (blocks in turn go to 8), by
+// the rows of weights and tokens that the `at` tiles read which a die computes at
+// once: few of them stay in its cache.  8192 x 512 x 3136 in tiles of 128 x 64:
+// 23.9 us together, 27.2 as they come; 8192 x 4096 x 4096 in such tiles 233 and
+// 185.
+bool tiles_together(int64_t nblocks, int64_t bn, int64_t bm, int64_t at) {
+  int64_t shared = 8;  // columns of tiles that fall to one die as they come
+  while (nblocks % shared) shared /= 2;
+  const int64_t apart =
+      std::min(nblocks / shared, at) * bn +
+      std::min(at, (8 * at + nblocks - 1) / nblocks) * bm;
+  const int64_t together =
+      std::min(nblocks, at) * bn + (at + nblocks - 1) / nblocks * bm;
+  return together < apart;
+}
+
 template <int WN, int WM, int NT, int MT, int S>
-bool launch_tiled(const DesInt8Product& p, bool together, hipStream_t stream) {
+bool launch_tiled(const DesInt8Product& p, int at, hipStream_t stream) {
   constexpr int BN = 32 * WN * NT, BM = 32 * WM * MT;
   constexpr int bytes = tiled_room(WN, WM, NT, MT, S) + BN * 8;
   const uint32_t nblocks = (p.N + (int64_t)BN - 1) / BN;
@@ -919,30 +937,26 @@ bool launch_tiled(const DesInt8Product& p, bool together, hipStream_t stream) {
                               hipFuncAttributeMaxDynamicSharedMemorySize,
                               bytes);
   hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(64 * WN * WM), bytes,
-                     stream, p, nblocks, mblocks, together);
+                     stream, p, nblocks, mblocks,
+                     tiles_together(nblocks, BN, BM, at));
   return true;
 }
 
 // The largest tiles that still give each of the chip's 256 units one (two of
-// 128 x 128).  Neighbouring tiles are computed on one die, whose cache then
-// reads their tokens once; with 8 or more tiles in a row of 256 x 256 ones the
-// order as it comes does that for the weights.  us:
+// 128 x 128); us:
 //                        256 x 256  128 x 128  128 x 64  64 x 64
-//   8192 x 4096 x 4096       130        152       182      215
-//   8192 x  512 x 3136        46         33        23       36
-//   4096 x 1024 x 2048        30         17        15       19
+//   8192 x 4096 x 4096       136        158       185      221
+//   8192 x  512 x 3136        47         28        24       29
+//   4096 x 1024 x 2048        29         16        14       18
 //   1024 x  512 x 3136        40         19        13        9
 bool choose_tiled(const DesInt8Product& p, hipStream_t stream) {
   auto tiles = [&](int64_t n, int64_t m) {
     return p.B * ((p.N + n - 1) / n) * ((p.M + m - 1) / m);
   };
-  if (tiles(256, 256) >= 256)
-    return launch_tiled<2, 4, 4, 2, 2>(p, p.N <= 7 * 256, stream);
-  if (tiles(128, 128) >= 512)
-    return launch_tiled<2, 2, 2, 2, 2>(p, true, stream);
-  if (tiles(128, 64) >= 256)
-    return launch_tiled<2, 2, 2, 1, 2>(p, true, stream);
-  return launch_tiled<2, 2, 1, 1, 3>(p, true, stream);
+  if (tiles(256, 256) >= 256) return launch_tiled<2, 4, 4, 2, 2>(p, 32, stream);
+  if (tiles(128, 128) >= 512) return launch_tiled<2, 2, 2, 2, 2>(p, 64, stream);
+  if (tiles(128, 64) >= 256) return launch_tiled<2, 2, 2, 1, 2>(p, 64, stream);
+  return launch_tiled<2, 2, 1, 1, 3>(p, 64, stream);
 }
 
 // codes -> rows every `step` bytes, with zeros behind them

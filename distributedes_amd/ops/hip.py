@@ -99,7 +99,8 @@ class HipOps:
         to x / scale, ties to even.  A row that holds a NaN or an infinity
         gets scale NaN and codes 0.
 
-        Fresh codes are a view whose rows begin at multiples of 16 bytes.
+        Fresh codes have rows that begin at multiples of 16 bytes, or of 128
+        where that adds 1/16 at most.
         out: (codes, scale) to write to; the codes' rows may lie anywhere
         apart from one another (bytes between them are left as they were)."""
         q, s = out if out is not None else (None, None)
@@ -135,4 +136,5 @@ class HipOps:
         where norm > max_norm, else 1; the norm stays on the GPU.  A NaN norm
         leaves the values as they are, an infinite one gives c = 0.
         out: tensors to write to (the tensors themselves clip in place)."""
-        return self.ext2.clip_by_global_norm(tensors, max_norm, out)
+        clipped, norm = self.ext2.clip_by_global_norm(tensors, max_norm, out)
+        return (clipped if out is None else list(out)), norm
