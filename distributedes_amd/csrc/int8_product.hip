@@ -244,8 +244,9 @@ __device__ void stage_block(const int8_t* x, int64_t xsr, int rows, int K,
 // token's codes from shared memory; L lanes' sums are joined at the row's end.
 //
 // The matrix instruction would want 16 rows in pieces of 64 bytes: for a layer
-// of 256 x 376 for each of 10000 members that reads 4.2 TB/s, this 6.1 (a plain
-// read of as much: 7.0), and rows of 3136 codes 5.1 against 6.3.
+// of 256 x 376 for each of 10000 members that reads 3.8 TB/s (254 us), this 6.1
+// (159 us; a plain read of as much: 7.0), and 2048 layers of 512 x 3136 4.6 TB/s
+// (709 us) against 6.4 (511 us).
 template <typename X, int MR, int U, bool ONCE>
 __global__ __launch_bounds__(256) void gemv_kernel(DesInt8Product p, int lbits,
                                                    int rows_a_wave) {
@@ -401,13 +402,15 @@ bool launch_gemv(const DesInt8Product& p, int lbits, int rows_a_wave,
 //  - up to 32 MB: latency counts.  A row to as many lanes as it fills, one load
 //    a row and turn, and as many waves as that gives, up to 8192.
 //  - weights that no cache would keep (256 MB), rows that begin on lines of
-//    128 bytes: past the caches, a line a turn and row.  K = 376 (rows of 384):
-//    4 lanes 292 us, 8 163, 16 167, 32 192; through the caches 180.
+//    128 bytes: past the caches, a line a turn and row.  K = 376 (rows of 384),
+//    960 MB: 4 lanes 293 us, 8 163, 16 167, 32 192; 503 MB by 8 lanes 82, and
+//    through the caches 90.
 //  - such weights in long rows that do not: 64 lanes, so that few lines are
-//    fetched in halves.  K = 3136: 509 us, 16 lanes 576.
+//    fetched in halves.  K = 3136, 3.3 GB: 509 us, 16 lanes 576, and through the
+//    caches 526.
 //  - all others: through the caches, which join halves of lines, and few lanes,
-//    which have fewer sums to join.  K = 200 (208): 2 lanes 255 us, 4 130, 8 104,
-//    16 99; past the caches 150.  K = 48: 1 lane 139, 2 124, 4 138.
+//    which have fewer sums to join.  503 MB, K = 300 (304): 2 lanes 223 us, 4 129,
+//    8 104, 16 99; past the caches 116.  K = 48: 1 lane 139, 2 124, 4 138.
 template <typename X, int MR>
 bool choose_gemv_rows(const DesInt8Product& p, hipStream_t stream) {
   const int64_t bytes = p.B * (int64_t)p.N * p.K;
@@ -747,11 +750,13 @@ __device__ __forceinline__ void tile_end(const DesInt8Product& p, int64_t b,
 // k = 16 * (lane >> 5), and holds the results of token (lane & 31) for channels
 // 8 * (i / 4) + 4 * (lane >> 5) + i % 4, i < 16.
 //
-// What bounds it: with 256 x 256 results a block, the matrix units' power (2.1
-// POPS on values as they occur, 5.0 by their clock); with fewer results the
-// reads of both operands, 20 bytes a clock and unit, and the barriers of a
-// stage.  Tried without gain: K shared by two groups of waves in a block, four
-// stages, priorities around the products.
+// What bounds it: with 256 x 256 results a block, the reads of shared memory (192
+// KB a stage at 64 bytes a clock: 3000 clocks, of which the matrix units work
+// 2048) and the clock, which falls from 2.4 to 2.0 GHz: 2.1 POPS.  With fewer
+// results a block, the loads of both operands (24 bytes a clock and unit) and the
+// barrier of a stage.  Tried without gain: 128 x 128 results a wave, K shared by
+// two groups of waves in a block, 3 or 4 stages, stages of 64, leaving a stage
+// before its last step, priorities around the products.
 template <int WN, int WM, int NT, int MT, int S>
 __global__ __launch_bounds__(64 * WN * WM) void tiled_kernel(
     DesInt8Product p, uint32_t nblocks, uint32_t mblocks, bool together) {
