@@ -103,13 +103,26 @@ __device__ __forceinline__ void store_past(T* p, const Vec<T, V>& v) {
   __builtin_nontemporal_store(t, reinterpret_cast<u32x4_any*>(p));
 }
 
-template <typename T, int N, bool PAST>
-__device__ void share_scale(const void* in, void* out, int64_t begin,
-                            int64_t end, double c, int tid) {
+// `factor()` joins the block for c; the first pieces are on their way meanwhile.
+template <typename T, int N, bool PAST, typename F>
+__device__ __forceinline__ void share_scale(const void* in, void* out,
+                                            int64_t begin, int64_t end,
+                                            F factor, int tid) {
   constexpr int V = 16 / sizeof(T);
   const T* p = (const T*)in;
   T* o = (T*)out;
   int64_t i = begin + tid * V;
+  Vec<T, V> t[4];
+  auto get = [&] {
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      t[u] = PAST ? load_past<T, V>(p + i + u * N * V)
+                  : *reinterpret_cast<const Vec<T, V>*>(p + i + u * N * V);
+  };
+  bool full = i + 3 * N * V + V <= end;
+  if (full) get();
+  const double c = factor();
+  if (c == 1.0 && in == out) return;  // in place, nothing to do
   auto put = [&](int64_t at, const Vec<T, V>& t) {
     Vec<T, V> r;
 #pragma unroll
@@ -118,14 +131,12 @@ __device__ void share_scale(const void* in, void* out, int64_t begin,
     if constexpr (PAST) store_past<T, V>(o + at, r);
     else *reinterpret_cast<Vec<T, V>*>(o + at) = r;
   };
-  for (; i + 3 * N * V + V <= end; i += 4 * N * V) {
-    Vec<T, V> t[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      t[u] = PAST ? load_past<T, V>(p + i + u * N * V)
-                  : *reinterpret_cast<const Vec<T, V>*>(p + i + u * N * V);
+  while (full) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) put(i + u * N * V, t[u]);
+    i += 4 * N * V;
+    full = i + 3 * N * V + V <= end;
+    if (full) get();
   }
   for (; i + V <= end; i += N * V)
     put(i, *reinterpret_cast<const Vec<T, V>*>(p + i));
@@ -147,19 +158,18 @@ __device__ double any_sum(const DesClipTable& t, int u, int64_t share,
   return share_sum<_Float16, N>(t.in[i], begin, end, tid);
 }
 
-template <int N, bool PAST>
-__device__ void any_scale(const DesClipTable& t, int u, int64_t share,
-                          double c, int tid) {
+template <int N, bool PAST, typename F>
+__device__ __forceinline__ void any_scale(const DesClipTable& t, int u,
+                                          int64_t share, F factor, int tid) {
   const int i = tensor_of(t, u);
-  if (c == 1.0 && t.in[i] == t.out[i]) return;  // in place, nothing to do
   const int64_t begin = (u - t.first[i]) * share;
   const int64_t end = min(begin + share, t.numel[i]);
   if (t.elem[i] == ELEM_F32)
-    share_scale<float, N, PAST>(t.in[i], t.out[i], begin, end, c, tid);
+    share_scale<float, N, PAST>(t.in[i], t.out[i], begin, end, factor, tid);
   else if (t.elem[i] == ELEM_BF16)
-    share_scale<Bf16, N, PAST>(t.in[i], t.out[i], begin, end, c, tid);
+    share_scale<Bf16, N, PAST>(t.in[i], t.out[i], begin, end, factor, tid);
   else
-    share_scale<_Float16, N, PAST>(t.in[i], t.out[i], begin, end, c, tid);
+    share_scale<_Float16, N, PAST>(t.in[i], t.out[i], begin, end, factor, tid);
 }
 
 __global__ __launch_bounds__(THREADS) void square_sums_kernel(
@@ -190,10 +200,12 @@ __global__ __launch_bounds__(THREADS) void scale_kernel(
     DesClipTable t, int64_t share, const double* __restrict__ sums, int n,
     double max_norm, float* __restrict__ norm, bool write_norm) {
   __shared__ double red[THREADS / 64];
-  const double v = norm_of(sums, n, red);
-  const double c = v > max_norm ? max_norm / v : 1.0;
-  if (write_norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)v;
-  any_scale<THREADS, PAST>(t, blockIdx.x, share, c, threadIdx.x);
+  auto factor = [&] {
+    const double v = norm_of(sums, n, red);
+    if (write_norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)v;
+    return v > max_norm ? max_norm / v : 1.0;
+  };
+  any_scale<THREADS, PAST>(t, blockIdx.x, share, factor, threadIdx.x);
 }
 
 // Norm and scaling of a few small tensors by one block, a wave for each share
@@ -214,7 +226,7 @@ __global__ __launch_bounds__(SMALL) void small_kernel(DesClipTable t,
   if (!scale) return;
   const double c = v > max_norm ? max_norm / v : 1.0;
   for (int u = wave; u < shares; u += SMALL / 64)
-    any_scale<64, false>(t, u, share, c, lane);
+    any_scale<64, false>(t, u, share, [&] { return c; }, lane);
 }
 
 }  // namespace
