@@ -40,7 +40,7 @@ def _check_codes(x, q, s):
     (65, 63), (5, 127), (11, 128), (3, 255), (6, 376), (4, 512), (2, 513),
     (3, 1023), (3, 1024), (2, 1025), (2, 2049), (2, 3136), (3, 4097),
     (2, 8193), (1, 16384), (1, 16385), (1, 40001), (2, 131072), (0, 8),
-    (8, 0)])
+    (8, 0), (600, 300), (513, 1100), (520, 4100), (515, 20003), (512, 33000)])
 def test_quantize_rows_sizes(ops, dtype, rows, cols):
     x = _rand(rows, cols, seed=rows + cols, dtype=dtype)
     _check_codes(x, *ops.quantize_rows(x))
@@ -145,7 +145,7 @@ def _check_both(ops, x, wq, sw, bias, act, out_dtype):
     (127, 257, 130), (128, 128, 128), (129, 256, 192), (200, 500, 1000),
     (255, 64, 4097), (256, 256, 256), (257, 255, 257), (300, 1, 300),
     (1000, 512, 3136), (1025, 513, 513), (3, 4096, 4096), (70, 40, 20000),
-    (5, 6, 131072), (600, 260, 0), (0, 4, 4), (4, 0, 4), (2500, 1, 1),
+    (5, 6, 131072), (600, 260, 0), (3, 5, 0), (4000, 4500, 0), (0, 4, 4), (4, 0, 4), (2500, 1, 1),
     (1, 3000, 77)])
 def test_product_sizes(ops, m, n, k):
     x = _rand(m, k, seed=m + n + k)
@@ -210,7 +210,7 @@ def test_member_products_of_more_tokens(ops, b, m, n, k, packed):
     (1, 1, 1, 1), (16, 1, 64, 64), (16, 1, 64, 4), (5, 1, 2, 64),
     (7, 1, 17, 256), (3, 1, 256, 376), (2, 2, 512, 3136), (3, 16, 33, 65),
     (4, 17, 40, 100), (2, 65, 130, 70), (3, 130, 129, 257), (2, 300, 300, 300),
-    (0, 1, 4, 4), (300, 1, 3, 3), (2, 5, 6, 70000), (70000, 1, 1, 3)])
+    (0, 1, 4, 4), (4, 1, 6, 0), (3, 40, 6, 0), (300, 1, 3, 3), (2, 5, 6, 70000), (70000, 1, 1, 3)])
 def test_member_product_sizes(ops, b, m, n, k):
     x = _rand(b, m, k, seed=b + m + n + k)
     wq, sw = _weights(ops, n, k, (b,))
@@ -346,6 +346,27 @@ def test_product_behind_32_bits(ops):
         assert not got[:-3].any()
 
 
+def test_product_larger_than_a_launch_is_refused(ops):
+    n = 70_000_000                # members of 64 threads: more than 2^32
+    wq = torch.ones(1, 1, 1, dtype=torch.int8, device="cuda").expand(n, 1, 1)
+    sw = torch.ones(1, 1, device="cuda").expand(n, 1)
+    x = torch.ones(1, 1, 1, device="cuda").expand(n, 1, 1)
+    with pytest.raises(ValueError, match="too large"):
+        ops.int8_linear(x, wq, sw)
+    got = ops.int8_linear(x[:60_000_000], wq[:60_000_000], sw[:60_000_000])
+    assert bool((got == 1).all())
+
+
+def test_no_gradient_mode_is_no_refusal(ops):
+    x = _rand(3, 8, seed=1).requires_grad_()
+    wq, sw = _weights(ops, 4, 8)
+    with torch.no_grad():
+        got = ops.int8_linear(x, wq, sw)
+    assert not got.requires_grad
+    with pytest.raises(ValueError):
+        ops.int8_linear(x, wq, sw)
+
+
 def test_product_same_bits_every_time(ops):
     for m, n, k in ((1, 700, 5000), (40, 64, 9000), (500, 300, 2000)):
         x, (wq, sw) = _rand(m, k, seed=1), _weights(ops, n, k)
@@ -429,6 +450,14 @@ def test_clip_extreme_values(ops, n):
         assert float(norm) == 0 and not got[0].any()
     got, norm = ops.clip_by_global_norm([_rand(n, seed=3)], 0.0)
     assert not got[0].any() and float(norm) > 0
+
+
+def test_clip_of_nothing(ops):
+    e = torch.empty(0, device="cuda")
+    for ts in ([e], [e, e.view(0, 3)], [e] * 120):
+        got, norm = ops.clip_by_global_norm(ts, 0.0, out=ts)
+        assert float(norm) == 0 and len(got) == len(ts)
+        assert float(ops.global_norm(ts)) == 0
 
 
 def test_clip_behind_32_bits(ops):
