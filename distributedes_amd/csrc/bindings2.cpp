@@ -212,6 +212,7 @@ std::pair<Tensor, Tensor> quantize_rows(const Tensor& x_,
                       "its last dimension");
     check_place(*q_, x_, "out[0]");
     check_place(*s_, x_, "out[1]");
+    check_no_grad(*s_, "out[1]");
     TORCH_CHECK_VALUE(as_rows(*q_, &r) && rows_apart(r, x_.size(-1)),
                       "out[0] must hold its rows apart, by two strides and "
                       "with a last stride of 1");

@@ -127,7 +127,8 @@ enum DesInt8Plan : int {
 };
 
 // Which kernel takes a product of M tokens, N channels and K codes for B
-// members.  A block of the first two holds its tokens' codes in shared memory.
+// members.  A stream of weights holds its tokens' codes in shared memory, the
+// next kernel only those that it makes from floats (des_int8_fused).
 // Tiles of 64 x 64 results leave the chip empty below about 100 of them: 128
 // tokens x 512 x 3136 take 5.2 us as a stream and 10 us in tiles, 1024 tokens
 // 15 and 10.7.

@@ -218,3 +218,17 @@ def test_cpu_tensors_are_refused_by_the_kernels():
                  lambda: ops.clip_by_global_norm([torch.zeros(3)], 1.0)):
         with pytest.raises(RuntimeError, match="GPU"):
             call()
+
+
+def test_every_refusal_is_listed():
+    assert len(_overlapping()) == 17
+
+
+def test_scales_that_require_a_gradient_are_not_written():
+    from distributedes_amd.ops.hip import HipOps, hip_available
+    if not hip_available():
+        pytest.skip("extension not built")
+    out = (torch.empty(3, 4, dtype=torch.int8),
+           torch.zeros(3, requires_grad=True))
+    with pytest.raises(ValueError, match="gradient"):
+        HipOps().quantize_rows(torch.zeros(3, 4), out=out)
