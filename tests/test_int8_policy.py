@@ -117,3 +117,12 @@ def test_checkpoint_round_trip(tmp_path):
     b.load_payload(load_checkpoint(str(tmp_path / "c.pt")))
     train_step(a), train_step(b)
     assert torch.equal(a.theta, b.theta)
+
+
+def test_command_line():
+    from distributedes_amd.__main__ import main
+    st = main(["--preset", "cartpole_es", "--ops", "torch_ref", "--set",
+               "pop=8", "generations=2", "episode_steps=10", "device=cpu",
+               "noise_table_size=65536", "precision=int8",
+               "max_grad_norm=0.5", "log_every=1000"])
+    assert st.generation == 2 and float(st.grad_norm) > 0
