@@ -135,7 +135,8 @@ std::vector<int64_t> lead_shape(const Tensor& x) {
 
 // Bytes from row to row of fresh codes: whole pieces of 16, which the products'
 // wide loads like, or whole lines of 128, where that adds 1/16 at most (a product
-// of 8192 x 512 x 3136 21.8 us instead of 23.9, with rows of 3200).
+// of 8192 x 512 x 3136 with rows of 3200 bytes: in tiles of 64 x 64 21.6 us instead
+// of 24.8, of 128 x 64 20.3 instead of 21.4, of 128 x 128 no difference).
 int64_t row_step(int64_t cols) {
   const int64_t line = (cols + 127) / 128 * 128;
   return line - cols <= cols / 16 ? line : (cols + 15) / 16 * 16;

@@ -754,9 +754,11 @@ __device__ __forceinline__ void tile_end(const DesInt8Product& p, int64_t b,
 // KB a stage at 64 bytes a clock: 3000 clocks, of which the matrix units work
 // 2048) and the clock, which falls from 2.4 to 2.0 GHz: 2.1 POPS.  With fewer
 // results a block, the loads of both operands (24 bytes a clock and unit) and the
-// barrier of a stage.  Tried without gain: 128 x 128 results a wave, K shared by
-// two groups of waves in a block, 3 or 4 stages, stages of 64, leaving a stage
-// before its last step, priorities around the products.
+// barrier of a stage; there, three stages and 8 waves hide more of them (128 x 128
+// results: 4 waves 25.0 us with two stages, 20.0 with three; 8 waves 22.8 and 17.7;
+// a fourth stage 18.0).  Tried without gain: 128 x 128 results a wave, K shared by
+// two groups of waves in a block, stages of 64, leaving a stage before its last
+// step, priorities around the products.
 template <int WN, int WM, int NT, int MT, int S>
 __global__ __launch_bounds__(64 * WN * WM) void tiled_kernel(
     DesInt8Product p, uint32_t nblocks, uint32_t mblocks, bool together) {
@@ -915,8 +917,8 @@ __global__ __launch_bounds__(64 * WN * WM) void tiled_kernel(
 // Whether neighbouring tiles are computed on one die (blocks in turn go to 8), by
 // the rows of weights and tokens that the `at` tiles read which a die computes at
 // once: few of them stay in its cache.  8192 x 512 x 3136 in tiles of 128 x 64:
-// 23.9 us together, 27.2 as they come; 8192 x 4096 x 4096 in such tiles 233 and
-// 185.
+// 25.5 us together, 27.6 as they come; 8192 x 4096 x 4096 in such tiles 290 and
+// 179.
 bool tiles_together(int64_t nblocks, int64_t bn, int64_t bm, int64_t at) {
   int64_t shared = 8;  // columns of tiles that fall to one die as they come
   while (nblocks % shared) shared /= 2;
@@ -947,21 +949,43 @@ bool launch_tiled(const DesInt8Product& p, int at, hipStream_t stream) {
   return true;
 }
 
-// The largest tiles that still give each of the chip's 256 units one (two of
-// 128 x 128); us:
-//                        256 x 256  128 x 128  128 x 64  64 x 64
-//   8192 x 4096 x 4096       136        158       185      221
-//   8192 x  512 x 3136        47         28        24       29
-//   4096 x 1024 x 2048        29         16        14       18
-//   1024 x  512 x 3136        40         19        13        9
+// The tiles that cost least, by their turns: a unit of the chip takes its tiles
+// one after the other (or two at once, half as fast), each with a time for a
+// stage of K and one for its end, in us.  Small tiles load more a result, large
+// ones leave units without work and nothing runs beside their ends.  Measured, us:
+//                        256 x 256  256 x 128  128 x 128  128 x 64  64 x 64
+//   8192 x 4096 x 4096       136                   158       185       221
+//   8192 x 2048 x 2048        31         37         34        45        52
+//   20000 x 1024 x 1000       37         35         29        36        39
+//   8192 x 1024 x 3136        52         29         34        43        53
+//   8192 x 1024 x 1024        19         14         13        16        18
+//   8192 x  512 x 3136        47                    18        21        22
+//   4096 x  512 x 3136        39         25         17        13        13
+//   1024 x  512 x 3136                              16        12         9
+// Three stages of 128 x 128 fill a unit's shared memory with one block: 18 us
+// instead of 23 for 8192 x 512 x 3136, a tile a unit; two blocks of two stages 34
+// instead of 37 for 8192 x 1024 x 3136, two a unit.
 bool choose_tiled(const DesInt8Product& p, hipStream_t stream) {
-  auto tiles = [&](int64_t n, int64_t m) {
-    return p.B * ((p.N + n - 1) / n) * ((p.M + m - 1) / m);
+  const int stages = (p.K + 127) / 128;
+  auto turns = [&](int64_t n, int64_t m) {
+    const int64_t tiles = p.B * ((p.N + n - 1) / n) * ((p.M + m - 1) / m);
+    return (tiles + 255) / 256;
   };
-  if (tiles(256, 256) >= 256) return launch_tiled<2, 4, 4, 2, 2>(p, 32, stream);
-  if (tiles(128, 128) >= 512) return launch_tiled<2, 2, 2, 2, 2>(p, 64, stream);
-  if (tiles(128, 64) >= 256) return launch_tiled<2, 2, 2, 1, 2>(p, 64, stream);
-  return launch_tiled<2, 2, 1, 1, 3>(p, 64, stream);
+  auto cost = [&](int64_t n, int64_t m, double stage, double end) {
+    return (double)turns(n, m) * (stage * stages + end);
+  };
+  const double by[5] = {cost(256, 256, 1.95, 5.0), cost(256, 128, 1.15, 3.5),
+                        cost(128, 128, 0.70, 0.5), cost(128, 64, 0.43, 0.3),
+                        cost(64, 64, 0.25, 0.2)};
+  switch (std::min_element(by, by + 5) - by) {
+    case 0: return launch_tiled<2, 4, 4, 2, 2>(p, 32, stream);
+    case 1: return launch_tiled<2, 4, 4, 1, 3>(p, 32, stream);
+    case 2:
+      if (turns(128, 128) == 1) return launch_tiled<2, 4, 2, 1, 3>(p, 32, stream);
+      return launch_tiled<2, 4, 2, 1, 2>(p, 64, stream);
+    case 3: return launch_tiled<2, 2, 2, 1, 3>(p, 64, stream);
+    default: return launch_tiled<2, 2, 1, 1, 3>(p, 64, stream);
+  }
 }
 
 // codes -> rows every `step` bytes, with zeros behind them

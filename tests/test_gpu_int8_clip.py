@@ -539,3 +539,24 @@ def test_mixed_places_are_refused(ops):
         ops.int8_linear(x, wq, sw, sw.cpu())
     with pytest.raises(ValueError):
         ops.clip_by_global_norm([x, x.cpu()], 1.0)
+
+
+@pytest.mark.parametrize("m,n,k", [
+    (8191, 1023, 2900), (16385, 510, 1290), (8190, 511, 700), (4095, 1000, 1900),
+    (8192, 512, 128), (8192, 512, 256), (8192, 512, 257), (8192, 512, 384),
+    (20001, 1020, 300), (4090, 500, 640), (4090, 500, 200), (2040, 500, 600),
+    (8190, 2040, 2000), (8190, 1022, 1100)])
+@pytest.mark.parametrize("out", [torch.float32, torch.float16])
+def test_product_tiles_by_turns(ops, m, n, k, out):
+    """Each size of tile with fewer stages than its ring and with many, a whole
+    last stage and a part of one, one turn and several."""
+    x = _rand(m, k, seed=m + n + k)
+    wq, sw = _weights(ops, n, k)
+    _check_both(ops, x, wq, sw, _rand(n, seed=2), "relu", out)
+
+
+@pytest.mark.parametrize("b,m,n,k", [
+    (40, 250, 500, 1000), (300, 250, 250, 900), (16, 500, 500, 2000),
+    (17, 500, 500, 2000), (30, 500, 500, 2000)])
+def test_member_product_tiles_by_turns(ops, b, m, n, k):
+    _sampled(ops, b, m, n, k)
