@@ -560,3 +560,30 @@ def test_product_tiles_by_turns(ops, m, n, k, out):
     (17, 500, 500, 2000), (30, 500, 500, 2000)])
 def test_member_product_tiles_by_turns(ops, b, m, n, k):
     _sampled(ops, b, m, n, k)
+
+
+@pytest.mark.parametrize("m,n,k", [(2040, 500, 601), (4090, 500, 641),
+                                   (8190, 511, 701), (8191, 1023, 2901),
+                                   (8190, 2040, 2001)])
+def test_captured_tiles_of_odd_rows(ops, m, n, k):
+    """Codes whose rows lie at odd addresses are copied inside the graph; two
+    graphs take turns with eager calls."""
+    g = torch.Generator("cuda").manual_seed(m)
+    codes = lambda r: torch.randint(-127, 128, (r, k), dtype=torch.int8,
+                                    device="cuda", generator=g)
+    wq, sw, sx = codes(n), torch.rand(n, device="cuda"), torch.rand(m, device="cuda")
+    xs = [codes(m), codes(m)]
+    ops.int8_matmul(xs[0], sx, wq, sw)
+    graphs = []
+    for x in xs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.int8_matmul(x, sx, wq, sw)
+        graphs.append((graph, out))
+    for _ in range(3):
+        for x, (graph, out) in zip(xs, graphs):
+            x.copy_(codes(m))
+            graph.replay()
+            want = ops.int8_matmul(x, sx, wq, sw)
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
