@@ -189,8 +189,10 @@ void launch_quantize(const Tensor& x, const Tensor& q, const Tensor& s) {
   CHECK_LAUNCH();
 }
 
-// x by two strides and a unit step, copied where it has other strides
+// x by two strides and a unit step, copied where it has other strides.  Without
+// elements any strides count as contiguous, and a copy would keep them.
 Tensor row_view(const Tensor& x) {
+  if (x.numel() == 0) return at::empty(x.sizes(), x.options());
   Rows r;
   return as_rows(x, &r) ? x : x.contiguous();
 }

@@ -587,3 +587,44 @@ def test_captured_tiles_of_odd_rows(ops, m, n, k):
             want = ops.int8_matmul(x, sx, wq, sw)
             torch.cuda.synchronize()
             assert torch.equal(out, want)
+
+
+# ------------------------------------------------------ rows of no values ---
+def _valueless(dtype):
+    """Rows of no values in layouts that dense tensors do not have."""
+    z = lambda *s: torch.zeros(*s, dtype=dtype, device="cuda")
+    return [z(3, 4, 5)[:, :2, :0], z(30, 40, 5)[:, :20, :0],
+            z(5, 9, 2)[::2, ::2, :0], z(2, 3, 4, 0).permute(2, 1, 0, 3),
+            z(7, 3)[::2, :0], z(600, 4, 2)[:, :2, :0]]
+
+
+@pytest.mark.parametrize("i", range(6))
+@pytest.mark.parametrize("act", ["none", "tanh"])
+def test_product_of_no_values_in_any_layout(ops, i, act):
+    sw, bias = _rand(6, seed=1), _rand(6, seed=2)
+    wq = torch.zeros(6, 0, dtype=torch.int8, device="cuda")
+    x, xq = _valueless(torch.float32)[i], _valueless(torch.int8)[i]
+    want = (bias.tanh() if act == "tanh" else bias).expand(*x.shape[:-1], 6)
+    out = torch.full(want.shape, 99.0, device="cuda")
+    ops.int8_linear(x, wq, sw, bias, act, out=out)
+    # the bias as it is, or its tanh: two steps of 32 bits
+    torch.testing.assert_close(out, want, rtol=4 * oracle.U32, atol=0)
+    out.fill_(99.0)
+    ops.int8_matmul(xq, torch.ones(x.shape[:-1], device="cuda"), wq, sw, bias,
+                    act, out=out)
+    torch.testing.assert_close(out, want, rtol=4 * oracle.U32, atol=0)
+
+
+@pytest.mark.parametrize("i", range(6))
+def test_quantize_rows_of_no_values_in_any_layout(ops, i):
+    x = _valueless(torch.float32)[i]
+    q, s = ops.quantize_rows(x)
+    assert q.shape == x.shape and q.dtype == torch.int8
+    assert s.shape == x.shape[:-1] and bool((s == 2.0 ** -126).all())
+    s = torch.zeros(x.shape[:-1], device="cuda")
+    ops.quantize_rows(x, out=(torch.empty(x.shape, dtype=torch.int8,
+                                          device="cuda"), s))
+    assert bool((s == 2.0 ** -126).all())
+    none = torch.zeros(4, 0, 6, 8, device="cuda").permute(2, 1, 0, 3)
+    q, s = ops.quantize_rows(none)             # no rows, by three strides
+    assert q.shape == none.shape and s.shape == none.shape[:-1]
