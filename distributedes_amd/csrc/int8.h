@@ -102,8 +102,8 @@ struct __attribute__((packed, aligned(sizeof(T)))) Vec { T v[V]; };
 // One batch of products, as the bindings pass it.  Strides in elements; the
 // elements of a row are next to each other.
 struct DesInt8Product {
-  const int8_t* x;      // [B, M, K]; null: xf is quantised on the way
-  const float* sx;      // [B, M]
+  const int8_t* x;      // [B, M, K]
+  const float* sx;      // [B, M]; null: xf is quantised on the way
   const void* xf;       // [B, M, K] float rows of type xelem
   const int8_t* w;      // [B, N, K]
   const float* sw;      // [B, N]

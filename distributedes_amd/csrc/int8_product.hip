@@ -1023,7 +1023,7 @@ extern "C" bool des_launch_int8_product(const DesInt8Product* p,
   const DesInt8Plan plan = des_int8_plan(q.B, q.M, q.N, q.K);
   if (plan == DES_INT8_TILED) return choose_tiled(q, stream);
   const bool gemv = plan == DES_INT8_GEMV;
-  if (q.x)
+  if (q.sx)  // not x, which is null where K = 0
     return gemv ? choose_gemv<int8_t>(q, stream)
                 : choose_stream<int8_t>(q, stream);
   if (q.xelem == ELEM_F32)

@@ -628,3 +628,19 @@ def test_quantize_rows_of_no_values_in_any_layout(ops, i):
     none = torch.zeros(4, 0, 6, 8, device="cuda").permute(2, 1, 0, 3)
     q, s = ops.quantize_rows(none)             # no rows, by three strides
     assert q.shape == none.shape and s.shape == none.shape[:-1]
+
+
+@pytest.mark.parametrize("lead,m", [((), 1), ((), 4), ((), 20), ((), 600),
+                                    ((3,), 2), ((3,), 20)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_scales_count_where_rows_have_no_values(ops, lead, m, bad):
+    """0 * NaN and 0 * inf: the token's results are NaN, as the twin's are."""
+    wq = torch.zeros(*lead, 6, 0, dtype=torch.int8, device="cuda")
+    sw, bias = _rand(*lead, 6, seed=1).abs(), _rand(*lead, 6, seed=2)
+    sx = torch.ones(*lead, m, device="cuda")
+    sx[..., -1] = bad
+    xq = torch.zeros(*lead, m, 0, dtype=torch.int8, device="cuda")
+    got = ops.int8_matmul(xq, sx, wq, sw, bias)
+    assert got[..., -1, :].isnan().all()
+    assert torch.equal(got[..., :-1, :],
+                       bias[..., None, :].expand(*lead, m - 1, 6))
