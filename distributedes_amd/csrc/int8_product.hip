@@ -12,6 +12,8 @@
 // operand, so that a lane's four results are four neighbouring channels of one
 // token: one store.
 #include <algorithm>
+#include <cfloat>
+#include <cmath>
 #include <type_traits>
 
 #include "int8.h"
@@ -52,9 +54,30 @@ __device__ __forceinline__ v4i load_tail(const int8_t* p, int left,
   return u.v;
 }
 
+// sum * sx * sw + b.  Sums stay below 2^31, so sum * sx stays in fp32's range for
+// sx below 2^96.  Under a larger one it may leave the range where the result does
+// not: 2^32 goes from sx to sw, both exactly.
+__device__ __forceinline__ bool large_scale(float sx) {
+  return fabsf(sx) >= 0x1p96f;
+}
+
+__device__ __forceinline__ float lowered(float sx) { return sx * 0x1p-32f; }
+
+// A finite sw stays finite: with a sum of 0 the result is b, with any other it is
+// beyond the range all the same.
+__device__ __forceinline__ float lifted(float sw) {
+  const float v = sw * 0x1p32f;
+  return fabsf(v) == INFINITY && fabsf(sw) < INFINITY ? copysignf(FLT_MAX, sw)
+                                                      : v;
+}
+
 __device__ __forceinline__ float finish(int sum, float sx, float sw, float b,
                                         int act) {
-  float v = (float)sum * sx * sw + b;
+  if (large_scale(sx)) {
+    sx = lowered(sx);
+    sw = lifted(sw);
+  }
+  float v = fmaf((float)sum * sx, sw, b);
   if (act == 1) v = v < 0.f ? 0.f : v;  // a NaN stays one
   if (act == 2) v = tanhf(v);
   return v;
@@ -655,8 +678,8 @@ __device__ __forceinline__ void tile_end(const DesInt8Product& p, int64_t b,
                                          const v16i (&acc)[NT][MT],
                                          const float (&sx)[MT],
                                          const float* sw, const float* bias,
-                                         int8_t* mine, int lane, int n0,
-                                         int m0) {
+                                         const float* lifts, int8_t* mine,
+                                         int lane, int n0, int m0) {
   constexpr int SIZE = V == 8 ? 2 : 4;            // of a value in shared memory
   constexpr int ROW = NT * 32 * SIZE + 16;        // bytes
   constexpr int LANES = NT * 32 / V, TOKENS = 64 / LANES;
@@ -668,17 +691,21 @@ __device__ __forceinline__ void tile_end(const DesInt8Product& p, int64_t b,
 #pragma unroll
     for (int ii = 0; ii < MT; ++ii) {
       if (i != ii) continue;
+      const bool large = large_scale(sx[ii]);
+      float st = large ? lowered(sx[ii]) : sx[ii];
+      asm volatile("" : "+v"(st));  // products of all i at once would spill
+      const float* sc = large ? lifts : sw;
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const int c = j * 32 + 8 * g + 4 * half;
-          const v4f s4 = *reinterpret_cast<const v4f*>(sw + c);
+          const v4f s4 = *reinterpret_cast<const v4f*>(sc + c);
           const v4f b4 = *reinterpret_cast<const v4f*>(bias + c);
           v4f v;
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            v[e] = fmaf((float)acc[j][ii][4 * g + e] * sx[ii], s4[e], b4[e]);
+            v[e] = fmaf((float)acc[j][ii][4 * g + e] * st, s4[e], b4[e]);
           int8_t* to = mine + row * ROW + c * SIZE;
           if constexpr (V == 8) {
             if (relu)
@@ -827,6 +854,7 @@ __global__ __launch_bounds__(64 * WN * WM) void tiled_kernel(
     if (c < BN) {
       factors[c] = sw[i];
       factors[BN + c] = bias[i];
+      factors[2 * BN + c] = lifted(sw[i]);
     }
   }
 
@@ -907,11 +935,11 @@ __global__ __launch_bounds__(64 * WN * WM) void tiled_kernel(
   const int nw = wn * NT * 32, mw = m0 + wm * MT * 32;
   int8_t* mine = shared + wave * tile_room(NT);
   if (p.out != ELEM_F32 && p.act != 2)
-    tile_end<NT, MT, 8>(p, b, acc, sx, factors + nw, factors + BN + nw, mine,
-                        lane, n0 + nw, mw);
+    tile_end<NT, MT, 8>(p, b, acc, sx, factors + nw, factors + BN + nw,
+                        factors + 2 * BN + nw, mine, lane, n0 + nw, mw);
   else
-    tile_end<NT, MT, 4>(p, b, acc, sx, factors + nw, factors + BN + nw, mine,
-                        lane, n0 + nw, mw);
+    tile_end<NT, MT, 4>(p, b, acc, sx, factors + nw, factors + BN + nw,
+                        factors + 2 * BN + nw, mine, lane, n0 + nw, mw);
 }
 
 // Whether neighbouring tiles are computed on one die (blocks in turn go to 8), by
@@ -933,7 +961,7 @@ bool tiles_together(int64_t nblocks, int64_t bn, int64_t bm, int64_t at) {
 template <int WN, int WM, int NT, int MT, int S>
 bool launch_tiled(const DesInt8Product& p, int at, hipStream_t stream) {
   constexpr int BN = 32 * WN * NT, BM = 32 * WM * MT;
-  constexpr int bytes = tiled_room(WN, WM, NT, MT, S) + BN * 8;
+  constexpr int bytes = tiled_room(WN, WM, NT, MT, S) + BN * 12;
   const uint32_t nblocks = (p.N + (int64_t)BN - 1) / BN;
   const uint32_t mblocks = (p.M + (int64_t)BM - 1) / BM;
   const int64_t blocks = p.B * (int64_t)nblocks * mblocks;

@@ -135,9 +135,12 @@ class TorchOps:
             return y if out is None else out.copy_(y)
         # whole numbers below 2^53: the sums are exact in any order
         y = xq.to(torch.float64) @ wq.to(torch.float64).transpose(-1, -2)
-        y = y.to(torch.float32) * sx.unsqueeze(-1) * sw.unsqueeze(-2)
+        # 64 bits: sum * sx may leave fp32's range where the result does not
+        y = y * sx.to(torch.float64).unsqueeze(-1)
+        y = y * sw.to(torch.float64).unsqueeze(-2)
         if bias is not None:
-            y = y + bias.unsqueeze(-2)
+            y = y + bias.to(torch.float64).unsqueeze(-2)
+        y = y.to(torch.float32)
         if activation == "relu":
             y = y.clamp_min(0)
         elif activation == "tanh":

@@ -644,3 +644,49 @@ def test_scales_count_where_rows_have_no_values(ops, lead, m, bad):
     assert got[..., -1, :].isnan().all()
     assert torch.equal(got[..., :-1, :],
                        bias[..., None, :].expand(*lead, m - 1, 6))
+
+
+# ------------------------------------------------------------ large scales ---
+@pytest.mark.parametrize("lead,m,n,k", [
+    ((), 2, 40, 3136), ((), 3, 40, 500), ((), 16, 70, 700), ((), 16, 70, 100),
+    ((), 700, 700, 300), ((), 2100, 2100, 200), ((5,), 2, 40, 64),
+    ((5,), 20, 40, 64)])
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("act", ["none", "tanh"])
+def test_product_of_large_rows(ops, lead, m, n, k, out, act):
+    """Rows of 1e36 with weights of 1e-8: sums times the token's scale leave
+    fp32's range, results do not.  Other tokens of the batch keep their bits."""
+    x = _rand(*lead, m, k, seed=1)
+    wq, sw = ops.quantize_rows(_rand(*lead, n, k, seed=2) * 1e-8)
+    bias = _rand(*lead, n, seed=3)
+    alone = ops.int8_linear(x, wq, sw, bias, act, out)
+    x[..., ::2, :] *= 1e36
+    x[..., 0, :] = 1e36
+    wq[..., 0, :] = 127
+    q, s = oracle.codes_and_scale(x)
+    want, err = oracle.product(q, s, wq, sw, bias, act)
+    got = _check_both(ops, x, wq, sw, bias, act, out)
+    oracle.check_product(got, want, err, out)
+    # the first product is that of codes alone, so that no product is finite
+    # by chance: its sum times the scale is beyond 32 bits
+    assert 127.0 * 127.0 * k * float(s.max()) > 3.4e38
+    assert torch.equal(got[..., 1::2, 1:], alone[..., 1::2, 1:])
+
+
+@pytest.mark.parametrize("m,n", [(2, 4), (16, 4), (600, 700), (2100, 2100)])
+def test_product_of_large_scales_on_both_sides(ops, m, n):
+    """A sum of 0 gives the bias, any other one is beyond the range."""
+    xq = torch.full((m, 64), 127, dtype=torch.int8, device="cuda")
+    wq = torch.full((n, 64), 127, dtype=torch.int8, device="cuda")
+    wq[::2, ::2] = -127
+    sx, sw = (torch.full((r,), 2.0 ** 100, device="cuda") for r in (m, n))
+    sw[3] = math.nan
+    sx[1] = -sx[1]
+    bias = _rand(n, seed=1)
+    got = ops.int8_matmul(xq, sx, wq, sw, bias)
+    assert torch.equal(got[:, ::2], bias[::2].expand(m, len(bias[::2])))
+    assert got[:, 3].isnan().all()
+    assert bool((got[1, 1] == -math.inf) & (got[0, 1] == math.inf))
+    sw[1] = 2.0 ** -126                        # 64 * 127^2 * 2^-26
+    got = ops.int8_matmul(xq, sx, wq, sw)
+    assert bool((got[::2, 1] == 127.0 ** 2 * 2.0 ** -20).all())

@@ -232,3 +232,22 @@ def test_scales_that_require_a_gradient_are_not_written():
            torch.zeros(3, requires_grad=True))
     with pytest.raises(ValueError, match="gradient"):
         HipOps().quantize_rows(torch.zeros(3, 4), out=out)
+
+
+@pytest.mark.parametrize("members", [0, 3])
+def test_products_of_large_rows(ref, members):
+    """Sums times the token's scale leave fp32's range, results do not."""
+    g = torch.Generator().manual_seed(5)
+    lead = (members,) if members else ()
+    x = torch.randn(*lead, 7, 3000, generator=g) * 1e36
+    x[..., 0, :] = 1e36
+    x[..., -1, :] = 1e-3
+    wq, sw = ref.quantize_rows(torch.randn(*lead, 9, 3000, generator=g) * 1e-8)
+    wq[..., 0, :] = 127
+    b = torch.randn(*lead, 9, generator=g)
+    xq, sx = ref.quantize_rows(x)
+    assert 127.0 * 127.0 * 3000 * float(sx.max()) > 3.4e38
+    want, err = oracle.product(xq, sx, wq, sw, b, "none")
+    assert bool((want.abs() < 3e38).all())
+    oracle.check_product(ref.int8_matmul(xq, sx, wq, sw, b), want, err,
+                         torch.float32)
