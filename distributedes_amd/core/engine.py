@@ -111,6 +111,9 @@ class TrainState:
         want_hip = (ops_backend != "torch_ref")
         self.ops = _make_ops(self.device, want_hip) if ops_backend != "torch_ref" \
             else _make_ops(torch.device("cpu"), False)
+        if self.ops.name == "hip" and (cfg.precision == "int8"
+                                       or cfg.max_grad_norm):
+            self.ops.ext2           # not built: raise before a generation runs
         table_dtype = (torch.bfloat16 if cfg.noise_dtype == "bf16"
                        else torch.float32)
         self.table = self.ops.fill_table(cfg.noise_table_size, self.table_seed,

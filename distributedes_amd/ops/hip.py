@@ -15,22 +15,27 @@ import torch
 _ext = None
 _ext2 = None
 _err = None
+_err2 = None
+
+
+def _import(name):
+    """(module, None) or (None, why not)."""
+    try:
+        return importlib.import_module("." + name, __package__), None
+    except ImportError as e:
+        try:
+            return importlib.import_module(name), None
+        except ImportError:
+            return None, e
 
 
 def _load():
-    global _ext, _ext2, _err
-    if _ext is not None or _err is not None:
-        return _ext
-    try:
-        # built in-tree; _hip_ops2: 8-bit rows and products, gradient norm
-        from . import _hip_ops, _hip_ops2
-        _ext, _ext2 = _hip_ops, _hip_ops2
-    except ImportError as e:
-        try:
-            _ext2 = importlib.import_module("_hip_ops2")
-            _ext = importlib.import_module("_hip_ops")
-        except ImportError:
-            _err = e
+    global _ext, _ext2, _err, _err2
+    if _ext is None and _err is None:
+        _ext, _err = _import("_hip_ops")
+        # 8-bit rows and products, gradient norm: whoever calls none of them
+        # does without it
+        _ext2, _err2 = _import("_hip_ops2")
     return _ext
 
 
@@ -50,9 +55,15 @@ class HipOps:
 
     def __init__(self):
         self.ext = _load()
-        self.ext2 = _ext2
         if self.ext is None:
             raise RuntimeError(f"HIP extension not built: {_err}")
+
+    @property
+    def ext2(self):
+        if _ext2 is None:
+            raise RuntimeError("HIP extension for 8-bit rows and gradient "
+                               f"norms (_hip_ops2) not built: {_err2}")
+        return _ext2
 
     # K1
     def fill_table(self, size: int, seed: int, device,
