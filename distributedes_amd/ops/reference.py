@@ -21,7 +21,14 @@ def _want(ok, message):
         raise ValueError(message)
 
 
+def _want_no_grad(**tensors):
+    for name, t in tensors.items():
+        _want(t is None or not (t.requires_grad and torch.is_grad_enabled()),
+              f"{name} requires a gradient, and this operator has none")
+
+
 def _want_product(x, wq, sw, bias, activation, out_dtype, out):
+    _want_no_grad(x=x, sw=sw, bias=bias, out=out)
     _want(wq.dtype == torch.int8, "wq must be int8")
     _want(wq.dim() in (2, 3),
           "wq must be [channels, cols] or [members, channels, cols]")
@@ -101,7 +108,9 @@ class TorchOps:
         _want(x.dtype in _ELEMS, "x must be float32, bfloat16 or float16")
         _want(x.dim() >= 1, "x must have at least one dimension")
         _want(x.shape[-1] <= _MAX_COLS, f"rows of at most {_MAX_COLS} values")
+        _want_no_grad(x=x)
         if out is not None:
+            _want_no_grad(out=out[1])
             _want(out[0].dtype == torch.int8 and out[0].shape == x.shape,
                   "out[0] must be int8 of x's shape")
             _want(out[1].dtype == torch.float32
@@ -128,6 +137,7 @@ class TorchOps:
         _want(xq.dim() >= 1, "xq must have at least one dimension")
         _want(sx.dtype == torch.float32 and sx.shape == xq.shape[:-1],
               "sx must be float32 of xq's shape without its last dimension")
+        _want_no_grad(sx=sx)
         _want_product(xq, wq, sw, bias, activation, out_dtype, out)
         if xq.dim() == 1:                    # one row, no axis of rows
             y = self.int8_matmul(xq[None], sx[None], wq, sw, bias, activation,
@@ -162,6 +172,7 @@ class TorchOps:
         for t in tensors:
             _want(t.dtype in _ELEMS,
                   "tensors must be float32, bfloat16 or float16")
+            _want_no_grad(tensors=t)
         return torch.stack([t.to(torch.float64).square().sum()
                             for t in tensors]).sum().sqrt()
 
@@ -175,6 +186,7 @@ class TorchOps:
         clipped = [(t.to(torch.float64) * c).to(t.dtype) for t in tensors]
         if out is not None:
             for o, t in zip(out, clipped):
+                _want_no_grad(out=o)
                 _want(o.dtype == t.dtype and o.shape == t.shape,
                       "out must be of its tensor's type and shape")
                 o.copy_(t)

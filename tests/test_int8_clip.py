@@ -251,3 +251,29 @@ def test_products_of_large_rows(ref, members):
     assert bool((want.abs() < 3e38).all())
     oracle.check_product(ref.int8_matmul(xq, sx, wq, sw, b), want, err,
                          torch.float32)
+
+
+def _leaf(*shape):
+    return torch.ones(*shape, requires_grad=True)
+
+
+@pytest.mark.parametrize("call", [
+    lambda o: o.quantize_rows(_leaf(3, 4)),
+    lambda o: o.quantize_rows(torch.zeros(3, 4), out=(
+        torch.empty(3, 4, dtype=torch.int8), _leaf(3))),
+    lambda o: o.int8_linear(_leaf(3, 4), *_w()),
+    lambda o: o.int8_linear(torch.zeros(3, 4), _w()[0], _leaf(5)),
+    lambda o: o.int8_linear(torch.zeros(3, 4), *_w(), bias=_leaf(5)),
+    lambda o: o.int8_linear(torch.zeros(3, 4), *_w(), out=_leaf(3, 5)),
+    lambda o: o.int8_matmul(torch.zeros(3, 4, dtype=torch.int8), _leaf(3),
+                            *_w()),
+    lambda o: o.global_norm([torch.zeros(3), _leaf(3)]),
+    lambda o: o.clip_by_global_norm([_leaf(3)], 1.0),
+    lambda o: o.clip_by_global_norm([torch.zeros(3)], 1.0, out=[_leaf(3)]),
+])
+def test_gradients_are_refused_alike(any_ops, call):
+    with pytest.raises(ValueError, match="gradient"):
+        call(any_ops)
+    if any_ops.name != "hip":                  # without one nothing is lost
+        with torch.no_grad():
+            call(any_ops)
