@@ -27,6 +27,60 @@ def _want_no_grad(**tensors):
               f"{name} requires a gradient, and this operator has none")
 
 
+def _span(t):
+    """The bytes that a tensor spans: [begin, end)."""
+    if t.numel() == 0:
+        return t.data_ptr(), t.data_ptr()
+    last = sum((n - 1) * step for n, step in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _overlap(a, b):
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a0 < b1 and b0 < a1 and a0 < a1 and b0 < b1
+
+
+def _rows_apart(t):
+    """Whether a tensor that is written holds its rows apart from one another,
+    by two strides and with a last stride of 1."""
+    cols = t.shape[-1]
+    if cols > 1 and t.stride(-1) != 1:
+        return False
+    groups = []                              # (size, step), inside out
+    for n, step in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if n == 1:
+            continue
+        if groups and step == groups[-1][0] * groups[-1][1]:
+            groups[-1] = (groups[-1][0] * n, groups[-1][1])
+        else:
+            groups.append((n, step))
+    room = cols
+    for n, step in sorted((g for g in groups if g[0] > 1), key=lambda g: g[1]):
+        if step < room:
+            return False
+        room += step * (n - 1)
+    return len(groups) <= 2
+
+
+def _want_apart(tensors, out):
+    """A write may meet no other write, and no read but that of its own tensor,
+    in place."""
+    uses = []
+    for i, (t, o) in enumerate(zip(tensors, out)):
+        if o.numel():
+            uses.append((*_span(o), i, True))
+            if _span(t) != _span(o):
+                uses.append((*_span(t), i, False))
+    written = read = 0
+    for begin, end, i, write in sorted(uses):
+        _want(begin >= written and (not write or begin >= read),
+              f"out[{i}] overlaps another tensor")
+        if write:
+            written = max(written, end)
+        else:
+            read = max(read, end)
+
+
 def _want_product(x, wq, sw, bias, activation, out_dtype, out):
     _want_no_grad(x=x, sw=sw, bias=bias, out=out)
     _want(wq.dtype == torch.int8, "wq must be int8")
@@ -48,6 +102,9 @@ def _want_product(x, wq, sw, bias, activation, out_dtype, out):
     _want(out is None or (out.dtype == out_dtype and out.is_contiguous()
                           and out.shape == (*x.shape[:-1], wq.shape[-2])),
           "out must be contiguous, of out_dtype and of the result's shape")
+    _want(out is None or not any(_overlap(out, t) for t in (x, wq, sw, bias)
+                                 if t is not None),
+          "out overlaps an argument")
 
 
 class TorchOps:
@@ -114,9 +171,14 @@ class TorchOps:
             _want(out[0].dtype == torch.int8 and out[0].shape == x.shape,
                   "out[0] must be int8 of x's shape")
             _want(out[1].dtype == torch.float32
-                  and out[1].shape == x.shape[:-1],
-                  "out[1] must be float32 of x's shape without its last "
-                  "dimension")
+                  and out[1].shape == x.shape[:-1] and out[1].is_contiguous(),
+                  "out[1] must be contiguous float32 of x's shape without its "
+                  "last dimension")
+            _want(_rows_apart(out[0]),
+                  "out[0] must hold its rows apart, by two strides and with a "
+                  "last stride of 1")
+            _want(not (_overlap(out[0], x) or _overlap(out[1], x)
+                       or _overlap(*out)), "out overlaps x or itself")
         v = x.detach().to(torch.float64)
         top = (v.abs().amax(dim=-1) if x.shape[-1]
                else v.new_zeros(x.shape[:-1]))
@@ -139,6 +201,7 @@ class TorchOps:
               "sx must be float32 of xq's shape without its last dimension")
         _want_no_grad(sx=sx)
         _want_product(xq, wq, sw, bias, activation, out_dtype, out)
+        _want(out is None or not _overlap(out, sx), "out overlaps an argument")
         if xq.dim() == 1:                    # one row, no axis of rows
             y = self.int8_matmul(xq[None], sx[None], wq, sw, bias, activation,
                                  out_dtype)[0]
@@ -159,6 +222,7 @@ class TorchOps:
 
     def int8_linear(self, x, wq, sw, bias=None, activation="none",
                     out_dtype=torch.float32, out=None):
+        _want(out is None or not _overlap(out, x), "out overlaps an argument")
         return self.int8_matmul(*self.quantize_rows(x), wq, sw, bias,
                                 activation, out_dtype, out)
 
@@ -179,16 +243,19 @@ class TorchOps:
     def clip_by_global_norm(self, tensors, max_norm, out=None):
         norm = self._norm64(tensors)
         _want(max_norm >= 0, "max_norm must be at least 0")
-        _want(out is None or len(out) == len(tensors),
-              "out must hold as many tensors")
+        if out is not None:
+            _want(len(out) == len(tensors), "out must hold as many tensors")
+            for o, t in zip(out, tensors):
+                _want_no_grad(out=o)
+                _want(o.dtype == t.dtype and o.shape == t.shape
+                      and o.is_contiguous(),
+                      "out must be contiguous, of its tensor's type and shape")
+            _want_apart(tensors, out)
         c = torch.where(norm > max_norm, max_norm / norm,
                         torch.ones_like(norm))
         clipped = [(t.to(torch.float64) * c).to(t.dtype) for t in tensors]
         if out is not None:
             for o, t in zip(out, clipped):
-                _want_no_grad(out=o)
-                _want(o.dtype == t.dtype and o.shape == t.shape,
-                      "out must be of its tensor's type and shape")
                 o.copy_(t)
             clipped = list(out)
         return clipped, norm.to(torch.float32)

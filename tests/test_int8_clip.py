@@ -277,3 +277,48 @@ def test_gradients_are_refused_alike(any_ops, call):
     if any_ops.name != "hip":                  # without one nothing is lost
         with torch.no_grad():
             call(any_ops)
+
+
+@pytest.mark.parametrize("i", range(17))
+def test_refused_by_the_twin(ref, i):
+    with pytest.raises(ValueError):
+        _overlapping()[i](ref)
+
+
+@pytest.mark.parametrize("call", [
+    lambda o: o.clip_by_global_norm([torch.zeros(2, 4)], 1.0,
+                                    out=[torch.zeros(4, 2).t()]),
+    lambda o: o.quantize_rows(torch.zeros(3, 4), out=(
+        torch.empty(3, 4, dtype=torch.int8), torch.zeros(6)[::2])),
+    lambda o: (lambda y: o.int8_matmul(
+        torch.zeros(4, 4, dtype=torch.int8), y.view(-1)[2:6],
+        *_w(4), out=y))(torch.zeros(4, 4)),
+])
+def test_outputs_refused_alike(any_ops, call):
+    with pytest.raises(ValueError):
+        call(any_ops)
+
+
+def test_nothing_is_written_where_one_output_is_refused(ref):
+    good, bad = torch.full((3,), 9.0), torch.zeros(4)
+    with pytest.raises(ValueError):
+        ref.clip_by_global_norm([torch.ones(3)] * 2, 1.0, out=[good, bad])
+    assert bool((good == 9).all())
+
+
+def test_the_twin_takes_what_lies_apart(ref):
+    """In place, side by side, rows between bytes that stay."""
+    buf = torch.arange(1.0, 9.0)
+    ts = [buf[:3], buf[3:3], buf[3:]]
+    want, norm = oracle.clipped(ts, 1.0)
+    got, n = ref.clip_by_global_norm(ts, 1.0, out=ts)
+    oracle.check_clipped(got, n, want, norm)
+    x = torch.randn(2, 3, 4, generator=torch.Generator().manual_seed(1))
+    store = torch.full((64,), 99, dtype=torch.int8)
+    for shape in ((24, 8, 1), (4, 8, 1), (30, 4, 1)):
+        q, s = store.as_strided((2, 3, 4), shape, 1), torch.empty(2, 3)
+        ref.quantize_rows(x, out=(q, s))
+        wq, ws = oracle.codes_and_scale(x)
+        assert torch.equal(q, wq) and torch.equal(s, ws)
+        q.fill_(99)
+        assert bool((store == 99).all())
