@@ -69,6 +69,10 @@ void check_place(const Tensor& t, const Tensor& like, const char* what) {
                     ", other arguments are on ", like.device());
 }
 
+// Counts a write that autograd does not see by itself: a graph that saved the
+// tensor then refuses to use it, instead of giving a wrong gradient.
+void mark_written(const Tensor& t) { t.unsafeGetTensorImpl()->bump_version(); }
+
 void check_gpu(const Tensor& t) {
   TORCH_CHECK(t.is_cuda(), "the HIP kernels need tensors on a GPU, not on ",
               t.device());
@@ -234,6 +238,10 @@ std::pair<Tensor, Tensor> quantize_rows(const Tensor& x_,
   as_rows(q, &qr);
   if (xr.lead != 1 && qr.lead != 1 && (xr.lead != qr.lead || xr.rows != qr.rows))
     x = x.contiguous();  // rows grouped unlike those of out
+  if (q_.has_value()) {
+    mark_written(q);
+    mark_written(s);
+  }
   launch_quantize(x, q, s);
   return {q, s};
 }
@@ -331,6 +339,7 @@ Tensor product(const Tensor& x_, const Tensor& sx_, const Tensor& wq_,
                const std::vector<int64_t>& shape) {
   Tensor y =
       out.has_value() ? *out : at::empty(shape, sw_.options().dtype(out_dtype));
+  if (out.has_value()) mark_written(y);
   if (y.numel() == 0) return y;
   DesInt8Product p = {};
   const bool members = wq_.dim() == 3;
@@ -576,6 +585,7 @@ std::pair<optional<std::vector<Tensor>>, Tensor> clip_by_global_norm(
     return to;
   };
   for (size_t i = 0; i < tensors.size(); ++i) {
+    if (out.has_value()) mark_written((*out)[i]);
     in.push_back(tensors[i].contiguous());
     to.push_back(out.has_value() ? (*out)[i] : at::empty_like(in[i]));
   }

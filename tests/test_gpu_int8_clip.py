@@ -690,3 +690,39 @@ def test_product_of_large_scales_on_both_sides(ops, m, n):
     sw[1] = 2.0 ** -126                        # 64 * 127^2 * 2^-26
     got = ops.int8_matmul(xq, sx, wq, sw)
     assert bool((got[::2, 1] == 127.0 ** 2 * 2.0 ** -20).all())
+
+
+# ---------------------------------------------------------------- autograd ---
+def test_writes_count_as_writes(ops):
+    """Version counters, as torch's own in-place operators keep them."""
+    x, (wq, sw) = _rand(3, 8, seed=1), _weights(ops, 4, 8)
+    q, s = ops.quantize_rows(x)
+    y, g, e = _rand(3, 4), _rand(5), torch.empty(0, 4, device="cuda")
+    for call, written in (
+            (lambda: ops.quantize_rows(x, out=(q, s)), (q, s)),
+            (lambda: ops.int8_linear(x, wq, sw, out=y), (y,)),
+            (lambda: ops.int8_matmul(q, s, wq, sw, out=y), (y,)),
+            (lambda: ops.int8_linear(x[:0], wq, sw, out=e), (e,)),
+            (lambda: ops.clip_by_global_norm([g, y], 1.0, out=[g, y]), (g, y)),
+            (lambda: ops.clip_by_global_norm([g], 9.0, out=[g]), (g,))):
+        before = [t._version for t in (x, q, s, y, g, e, wq, sw)]
+        call()
+        for t, v in zip((x, q, s, y, g, e, wq, sw), before):
+            assert t._version == v + any(t is w for w in written)
+
+
+def test_a_saved_tensor_that_is_written_is_noticed(ops):
+    leaf = _rand(5, seed=2).requires_grad_()
+    for write in (lambda t: ops.clip_by_global_norm([t], 0.1, out=[t]),
+                  lambda t: ops.int8_linear(
+                      _rand(1, 8), *_weights(ops, 5, 8), out=t[None])):
+        saved = _rand(5, seed=3)
+        loss = (leaf * saved).sum()
+        write(saved)
+        with pytest.raises(RuntimeError, match="inplace"):
+            loss.backward()
+    with torch.inference_mode():
+        t = _rand(5, seed=4)
+        ops.clip_by_global_norm([t], 0.1, out=[t])      # has no counter
+    with pytest.raises(RuntimeError, match="nference"):
+        ops.clip_by_global_norm([t], 0.1, out=[t])
