@@ -59,9 +59,13 @@ int elem_of(at::ScalarType t, const char* what) {
                     t);
 }
 
+// A tangent of forward mode would be lost as well, also where gradients are off.
 void check_no_grad(const Tensor& t, const char* what) {
   TORCH_CHECK_VALUE(!(t.requires_grad() && at::GradMode::is_enabled()), what,
                     " requires a gradient, and this operator has none");
+  TORCH_CHECK_VALUE(!t._fw_grad(0).defined(), what,
+                    " carries a forward-mode gradient, and this operator has "
+                    "none");
 }
 
 void check_place(const Tensor& t, const Tensor& like, const char* what) {

@@ -8,6 +8,7 @@ index tensors beyond `chunk` rows.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from ..core import noise as noise_mod
 
@@ -25,6 +26,9 @@ def _want_no_grad(**tensors):
     for name, t in tensors.items():
         _want(t is None or not (t.requires_grad and torch.is_grad_enabled()),
               f"{name} requires a gradient, and this operator has none")
+        _want(t is None or forward_ad.unpack_dual(t).tangent is None,
+              f"{name} carries a forward-mode gradient, and this operator has "
+              "none")
 
 
 def _span(t):

@@ -322,3 +322,27 @@ def test_the_twin_takes_what_lies_apart(ref):
         assert torch.equal(q, wq) and torch.equal(s, ws)
         q.fill_(99)
         assert bool((store == 99).all())
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_gradients_are_refused_alike(any_ops, grad):
+    import torch.autograd.forward_ad as forward_ad
+    z = torch.zeros
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        dual = lambda *s: forward_ad.make_dual(z(*s), torch.ones(*s))
+        for call in (
+                lambda: any_ops.quantize_rows(dual(3, 4)),
+                lambda: any_ops.quantize_rows(z(3, 4), out=(
+                    z(3, 4, dtype=torch.int8), dual(3))),
+                lambda: any_ops.int8_linear(dual(3, 4), *_w()),
+                lambda: any_ops.int8_linear(z(3, 4), _w()[0], dual(5)),
+                lambda: any_ops.int8_linear(z(3, 4), *_w(), bias=dual(5)),
+                lambda: any_ops.int8_linear(z(3, 4), *_w(), out=dual(3, 5)),
+                lambda: any_ops.int8_matmul(z(3, 4, dtype=torch.int8),
+                                            dual(3), *_w()),
+                lambda: any_ops.global_norm([dual(3)]),
+                lambda: any_ops.clip_by_global_norm([z(3), dual(3)], 1.0),
+                lambda: any_ops.clip_by_global_norm([z(3)], 1.0,
+                                                    out=[dual(3)])):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
