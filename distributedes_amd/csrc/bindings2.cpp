@@ -77,6 +77,12 @@ void check_place(const Tensor& t, const Tensor& like, const char* what) {
 // tensor then refuses to use it, instead of giving a wrong gradient.
 void mark_written(const Tensor& t) { t.unsafeGetTensorImpl()->bump_version(); }
 
+// Kernels read memory as it is: a view that torch negates when it reads it is
+// written out first (resolve_neg), and none is written to.
+void check_plain(const Tensor& t, const char* what) {
+  TORCH_CHECK_VALUE(!t.is_neg(), what, " must not be a negated view");
+}
+
 void check_gpu(const Tensor& t) {
   TORCH_CHECK(t.is_cuda(), "the HIP kernels need tensors on a GPU, not on ",
               t.device());
@@ -223,6 +229,8 @@ std::pair<Tensor, Tensor> quantize_rows(const Tensor& x_,
                       "its last dimension");
     check_place(*q_, x_, "out[0]");
     check_place(*s_, x_, "out[1]");
+    check_plain(*q_, "out[0]");
+    check_plain(*s_, "out[1]");
     check_no_grad(*s_, "out[1]");
     TORCH_CHECK_VALUE(as_rows(*q_, &r) && rows_apart(r, x_.size(-1)),
                       "out[0] must hold its rows apart, by two strides and "
@@ -236,7 +244,7 @@ std::pair<Tensor, Tensor> quantize_rows(const Tensor& x_,
   Tensor q = q_.has_value() ? *q_ : new_codes(x_);
   Tensor s = s_.has_value() ? *s_
                             : at::empty(shape, x_.options().dtype(at::kFloat));
-  Tensor x = row_view(x_);
+  Tensor x = row_view(x_.resolve_neg());
   Rows xr, qr;
   as_rows(x, &xr);
   as_rows(q, &qr);
@@ -301,6 +309,7 @@ std::vector<int64_t> check_product(const Tensor& x, const Tensor& wq,
                       at::IntArrayRef(shape));
     check_place(*out, x, "out");
     check_no_grad(*out, "out");
+    check_plain(*out, "out");
     TORCH_CHECK_VALUE(!overlap(*out, x) && !overlap(*out, wq) &&
                           !overlap(*out, sw) &&
                           !(bias.has_value() && overlap(*out, *bias)),
@@ -347,7 +356,7 @@ Tensor product(const Tensor& x_, const Tensor& sx_, const Tensor& wq_,
   if (y.numel() == 0) return y;
   DesInt8Product p = {};
   const bool members = wq_.dim() == 3;
-  Tensor x = row_view(x_);
+  Tensor x = row_view(x_.resolve_neg());
   if (!members) {
     Rows r;
     as_rows(x, &r);
@@ -368,7 +377,7 @@ Tensor product(const Tensor& x_, const Tensor& sx_, const Tensor& wq_,
   const int64_t K = x.size(-1);
   Tensor sx;
   if (sx_.defined()) {
-    sx = sx_.contiguous();
+    sx = sx_.resolve_neg().contiguous();
   } else if (!des_int8_fused(p.M, K)) {
     const Tensor q = new_codes(x);
     sx = at::empty(lead_shape(x), x.options().dtype(at::kFloat));
@@ -385,16 +394,17 @@ Tensor product(const Tensor& x_, const Tensor& sx_, const Tensor& wq_,
     p.xf = x.data_ptr();
     p.xelem = elem_of(x.scalar_type(), "x");
   }
-  const Tensor wq =
-      K > 1 && wq_.stride(-1) != 1 ? wq_.contiguous() : wq_;
+  Tensor wq = wq_.resolve_neg();
+  if (K > 1 && wq.stride(-1) != 1) wq = wq.contiguous();
   TORCH_CHECK_VALUE(wq.size(-2) <= MAX_ROWS, "too many channels");
   p.N = (int32_t)wq.size(-2);
   p.K = (int32_t)K;
   p.wsb = members ? wq.stride(0) : 0;
   p.wsr = wq.stride(-2);
   p.wwhole = whole_rows(wq);
-  const Tensor sw = sw_.contiguous();
-  const Tensor bias = bias_.has_value() ? bias_->contiguous() : Tensor();
+  const Tensor sw = sw_.resolve_neg().contiguous();
+  const Tensor bias =
+      bias_.has_value() ? bias_->resolve_neg().contiguous() : Tensor();
   p.w = wq.data_ptr<int8_t>();
   p.sw = sw.data_ptr<float>();
   p.bias = bias.defined() ? bias.data_ptr<float>() : nullptr;
@@ -523,7 +533,8 @@ Tensor global_norm(const std::vector<Tensor>& tensors) {
   check_gpu(tensors[0]);
   const c10::DeviceGuard guard(tensors[0].device());
   std::vector<Tensor> in;
-  for (const Tensor& t : tensors) in.push_back(t.contiguous());
+  for (const Tensor& t : tensors)
+    in.push_back(t.resolve_neg().contiguous());
   const int64_t share = share_of(in);
   const Tables tables = tables_of(in, {}, share);
   Tensor norm = at::empty({}, in[0].options().dtype(at::kFloat));
@@ -567,6 +578,7 @@ std::pair<optional<std::vector<Tensor>>, Tensor> clip_by_global_norm(
                         "and shape");
       check_place(o, tensors[0], "out");
       check_no_grad(o, "out");
+      check_plain(o, "out");
       if (o.numel() == 0) continue;
       const auto a = span(tensors[i]), b = span(o);
       uses.push_back({b.first, b.second, i, true});
@@ -590,7 +602,7 @@ std::pair<optional<std::vector<Tensor>>, Tensor> clip_by_global_norm(
   };
   for (size_t i = 0; i < tensors.size(); ++i) {
     if (out.has_value()) mark_written((*out)[i]);
-    in.push_back(tensors[i].contiguous());
+    in.push_back(tensors[i].resolve_neg().contiguous());
     to.push_back(out.has_value() ? (*out)[i] : at::empty_like(in[i]));
   }
   const int64_t share = share_of(in);

@@ -31,6 +31,10 @@ def _want_no_grad(**tensors):
               "none")
 
 
+def _want_plain(*out):
+    _want(not any(o.is_neg() for o in out), "out must not be a negated view")
+
+
 def _span(t):
     """The bytes that a tensor spans: [begin, end)."""
     if t.numel() == 0:
@@ -106,6 +110,8 @@ def _want_product(x, wq, sw, bias, activation, out_dtype, out):
     _want(out is None or (out.dtype == out_dtype and out.is_contiguous()
                           and out.shape == (*x.shape[:-1], wq.shape[-2])),
           "out must be contiguous, of out_dtype and of the result's shape")
+    if out is not None:
+        _want_plain(out)
     _want(out is None or not any(_overlap(out, t) for t in (x, wq, sw, bias)
                                  if t is not None),
           "out overlaps an argument")
@@ -172,6 +178,7 @@ class TorchOps:
         _want_no_grad(x=x)
         if out is not None:
             _want_no_grad(out=out[1])
+            _want_plain(*out)
             _want(out[0].dtype == torch.int8 and out[0].shape == x.shape,
                   "out[0] must be int8 of x's shape")
             _want(out[1].dtype == torch.float32
@@ -251,6 +258,7 @@ class TorchOps:
             _want(len(out) == len(tensors), "out must hold as many tensors")
             for o, t in zip(out, tensors):
                 _want_no_grad(out=o)
+                _want_plain(o)
                 _want(o.dtype == t.dtype and o.shape == t.shape
                       and o.is_contiguous(),
                       "out must be contiguous, of its tensor's type and shape")

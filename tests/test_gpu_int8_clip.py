@@ -726,3 +726,34 @@ def test_a_saved_tensor_that_is_written_is_noticed(ops):
         ops.clip_by_global_norm([t], 0.1, out=[t])      # has no counter
     with pytest.raises(RuntimeError, match="nference"):
         ops.clip_by_global_norm([t], 0.1, out=[t])
+
+
+# ----------------------------------------------------------- negated views ---
+def _negated(t):
+    """t as a view of -t's memory that torch negates when it reads it; its last
+    stride is 2."""
+    view = torch.complex(torch.zeros_like(t), -t).conj().imag
+    assert view.is_neg() and torch.equal(view, t)
+    return view
+
+
+def test_negated_views_are_read_as_their_values(ops):
+    x = _rand(5, 1, seed=1)                # rows of one value: any last stride
+    v = _negated(x)
+    _check_codes(x, *ops.quantize_rows(v))
+    wq, sw = _weights(ops, 4, 1)
+    bias = _rand(4, seed=2)
+    assert torch.equal(ops.int8_linear(v, wq, sw, bias),
+                       ops.int8_linear(x, wq, sw, bias))
+    xq, sx = ops.quantize_rows(x)
+    want = ops.int8_matmul(xq, sx, wq, sw, bias)
+    one = slice(0, 1)                      # a vector of one value: contiguous
+    assert torch.equal(want[:, one], ops.int8_matmul(
+        xq, sx, wq[one], _negated(sw[one]), _negated(bias[one])))
+    assert torch.equal(want[one], ops.int8_matmul(xq[one], _negated(sx[one]),
+                                                  wq, sw, bias))
+    t = _rand(1, seed=3)
+    for norm in (0.1, 9.0):
+        got, n = ops.clip_by_global_norm([_negated(t), x], norm)
+        oracle.check_clipped(got, n, *oracle.clipped([t, x], norm))
+    assert torch.equal(ops.global_norm([_negated(t), _negated(x)]), n)

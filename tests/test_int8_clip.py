@@ -346,3 +346,24 @@ def test_forward_mode_gradients_are_refused_alike(any_ops, grad):
                                                     out=[dual(3)])):
             with pytest.raises(ValueError, match="forward-mode"):
                 call()
+
+
+def _negated(t):
+    """A view of -t's memory that torch negates when it reads it."""
+    view = torch.complex(torch.zeros_like(t, dtype=torch.float32),
+                         -t.float()).conj().imag
+    assert view.is_neg()
+    return view
+
+
+@pytest.mark.parametrize("call", [
+    lambda o: o.quantize_rows(torch.zeros(3, 1), out=(
+        torch.empty(3, 1, dtype=torch.int8), _negated(torch.ones(1)).expand(3))),
+    lambda o: o.int8_linear(torch.zeros(1, 4), *_w(1),
+                            out=_negated(torch.zeros(1, 1))),
+    lambda o: o.clip_by_global_norm([torch.zeros(1)], 1.0,
+                                    out=[_negated(torch.zeros(1))]),
+])
+def test_negated_views_are_not_written(any_ops, call):
+    with pytest.raises(ValueError):
+        call(any_ops)
