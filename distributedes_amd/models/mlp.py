@@ -100,5 +100,8 @@ class Int8Layers:
             e = spec._by_name[name + ".bias"]
             b.copy_(flat[:, e.offset:e.offset + e.numel])
 
-    def data_ptr(self) -> int:
-        return self.codes[0].data_ptr()
+    def graph_key(self) -> tuple:
+        """What a captured graph has of these weights: all buffers' addresses,
+        and the form that it reads them in."""
+        return (self.shared, *(t.data_ptr() for t in self.codes + self.scales
+                               + self.biases))

@@ -321,7 +321,9 @@ class HipRollout:
                      and self.device.type == "cuda"
                      and not getattr(self, "_graphs_broken", False))
         if use_graph:
-            key = (episode_steps, pop_w.data_ptr(), id(normalizer), observe)
+            weights = (pop_w.graph_key() if isinstance(pop_w, Int8Layers)
+                       else pop_w.data_ptr())
+            key = (episode_steps, weights, id(normalizer), observe)
             g = self._graphs.get(key)
             if g is None:
                 try:

@@ -95,3 +95,33 @@ def test_evaluation_in_8_bits(episodes):
     a, b = (evaluate(st, episodes=episodes) for _ in range(2))
     assert a == b and a["env_steps"] == episodes * 20
     assert a["return_min"] <= a["return_mean"] <= a["return_max"]
+
+
+@pytest.mark.parametrize("shared", [False, True])
+def test_graphs_are_told_apart_by_all_buffers(shared):
+    """Weights that share one buffer with weights of an earlier graph, and are
+    others, get a graph of their own."""
+    st = TrainState(_cfg("humanoid_es_10k", episode_steps=4))
+    g = torch.Generator("cuda").manual_seed(1)
+    P = 64
+
+    def layers(shared):
+        out = Int8Layers(st.model, P, "cuda", shared=shared)
+        flat = torch.randn(1 if shared else P, st.dim, generator=g,
+                           device="cuda") * 0.1
+        out.load(st.ops, flat)
+        return out
+
+    a, b = layers(False), layers(shared)
+    a.codes[0][:1].copy_(b.codes[0][:1])
+    b.codes[0] = a.codes[0][:b.codes[0].shape[0]]
+    ids = torch.arange(P)
+    got = {}
+    for graph in (True, False):
+        for name, w in (("a", a), ("b", b)):
+            got[name, graph] = st._hip_rollout.run(
+                w, 7, ids, 4, st.normalizer, allow_graph=graph,
+                observe=False)[0]
+    assert not torch.equal(got["a", False], got["b", False])
+    for name in "ab":
+        assert torch.equal(got[name, True], got[name, False])
