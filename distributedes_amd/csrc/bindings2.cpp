@@ -110,6 +110,11 @@ struct Rows {
 
 bool as_rows(const Tensor& t, Rows* r) {
   const int64_t last = t.dim() - 1;
+  for (int64_t d = 0; d < last; ++d)
+    if (t.size(d) == 0) {  // no rows: any strides will do
+      *r = Rows{1, 0, 0, 0};
+      return true;
+    }
   if (t.size(last) > 1 && t.stride(last) != 1) return false;
   int64_t size[2] = {1, 1}, step[2] = {0, 0};
   int used = 0;  // from the inside out

@@ -52,6 +52,8 @@ def _rows_apart(t):
     """Whether a tensor that is written holds its rows apart from one another,
     by two strides and with a last stride of 1."""
     cols = t.shape[-1]
+    if 0 in t.shape[:-1]:                    # no rows
+        return True
     if cols > 1 and t.stride(-1) != 1:
         return False
     groups = []                              # (size, step), inside out

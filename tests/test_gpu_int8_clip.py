@@ -757,3 +757,19 @@ def test_negated_views_are_read_as_their_values(ops):
         got, n = ops.clip_by_global_norm([_negated(t), x], norm)
         oracle.check_clipped(got, n, *oracle.clipped([t, x], norm))
     assert torch.equal(ops.global_norm([_negated(t), _negated(x)]), n)
+
+
+@pytest.mark.parametrize("shape,perm", [
+    ((3, 0, 0, 17), (0, 1, 2, 3)), ((0, 0, 5, 8), (2, 0, 1, 3)),
+    ((4, 0, 6, 8), (2, 1, 0, 3)), ((3, 0, 0, 2, 0), (3, 1, 0, 2, 4)),
+    ((0, 9, 4), (0, 2, 1))])
+def test_no_rows_in_any_layout(ops, shape, perm):
+    x = torch.zeros(shape, device="cuda").permute(perm)
+    q, s = ops.quantize_rows(x)
+    assert q.shape == x.shape and s.shape == x.shape[:-1]
+    out = (torch.zeros(shape, dtype=torch.int8, device="cuda").permute(perm), s)
+    assert ops.quantize_rows(x, out=out)[0].shape == x.shape
+    wq, sw = _weights(ops, 5, max(1, x.shape[-1]))
+    wq = wq[:, :x.shape[-1]]
+    assert ops.int8_linear(x, wq, sw).shape == (*x.shape[:-1], 5)
+    assert ops.int8_matmul(q, s, wq, sw).shape == (*x.shape[:-1], 5)
