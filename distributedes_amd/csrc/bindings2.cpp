@@ -78,7 +78,10 @@ void check_place(const Tensor& t, const Tensor& like, const char* what) {
 void mark_written(const Tensor& t) { t.unsafeGetTensorImpl()->bump_version(); }
 
 // Kernels read memory as it is: a view that torch negates when it reads it is
-// written out first (resolve_neg), and none is written to.
+// written out first, and none is written to.  (resolve_neg alone goes through torch's
+// dispatcher where there is nothing to do, too.)
+Tensor plain(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 void check_plain(const Tensor& t, const char* what) {
   TORCH_CHECK_VALUE(!t.is_neg(), what, " must not be a negated view");
 }
@@ -249,7 +252,7 @@ std::pair<Tensor, Tensor> quantize_rows(const Tensor& x_,
   Tensor q = q_.has_value() ? *q_ : new_codes(x_);
   Tensor s = s_.has_value() ? *s_
                             : at::empty(shape, x_.options().dtype(at::kFloat));
-  Tensor x = row_view(x_.resolve_neg());
+  Tensor x = row_view(plain(x_));
   Rows xr, qr;
   as_rows(x, &xr);
   as_rows(q, &qr);
@@ -361,7 +364,7 @@ Tensor product(const Tensor& x_, const Tensor& sx_, const Tensor& wq_,
   if (y.numel() == 0) return y;
   DesInt8Product p = {};
   const bool members = wq_.dim() == 3;
-  Tensor x = row_view(x_.resolve_neg());
+  Tensor x = row_view(plain(x_));
   if (!members) {
     Rows r;
     as_rows(x, &r);
@@ -382,7 +385,7 @@ Tensor product(const Tensor& x_, const Tensor& sx_, const Tensor& wq_,
   const int64_t K = x.size(-1);
   Tensor sx;
   if (sx_.defined()) {
-    sx = sx_.resolve_neg().contiguous();
+    sx = plain(sx_).contiguous();
   } else if (!des_int8_fused(p.M, K)) {
     const Tensor q = new_codes(x);
     sx = at::empty(lead_shape(x), x.options().dtype(at::kFloat));
@@ -399,7 +402,7 @@ Tensor product(const Tensor& x_, const Tensor& sx_, const Tensor& wq_,
     p.xf = x.data_ptr();
     p.xelem = elem_of(x.scalar_type(), "x");
   }
-  Tensor wq = wq_.resolve_neg();
+  Tensor wq = plain(wq_);
   if (K > 1 && wq.stride(-1) != 1) wq = wq.contiguous();
   TORCH_CHECK_VALUE(wq.size(-2) <= MAX_ROWS, "too many channels");
   p.N = (int32_t)wq.size(-2);
@@ -407,9 +410,9 @@ Tensor product(const Tensor& x_, const Tensor& sx_, const Tensor& wq_,
   p.wsb = members ? wq.stride(0) : 0;
   p.wsr = wq.stride(-2);
   p.wwhole = whole_rows(wq);
-  const Tensor sw = sw_.resolve_neg().contiguous();
+  const Tensor sw = plain(sw_).contiguous();
   const Tensor bias =
-      bias_.has_value() ? bias_->resolve_neg().contiguous() : Tensor();
+      bias_.has_value() ? plain(*bias_).contiguous() : Tensor();
   p.w = wq.data_ptr<int8_t>();
   p.sw = sw.data_ptr<float>();
   p.bias = bias.defined() ? bias.data_ptr<float>() : nullptr;
@@ -539,7 +542,7 @@ Tensor global_norm(const std::vector<Tensor>& tensors) {
   const c10::DeviceGuard guard(tensors[0].device());
   std::vector<Tensor> in;
   for (const Tensor& t : tensors)
-    in.push_back(t.resolve_neg().contiguous());
+    in.push_back(plain(t).contiguous());
   const int64_t share = share_of(in);
   const Tables tables = tables_of(in, {}, share);
   Tensor norm = at::empty({}, in[0].options().dtype(at::kFloat));
@@ -607,7 +610,7 @@ std::pair<optional<std::vector<Tensor>>, Tensor> clip_by_global_norm(
   };
   for (size_t i = 0; i < tensors.size(); ++i) {
     if (out.has_value()) mark_written((*out)[i]);
-    in.push_back(tensors[i].resolve_neg().contiguous());
+    in.push_back(plain(tensors[i]).contiguous());
     to.push_back(out.has_value() ? (*out)[i] : at::empty_like(in[i]));
   }
   const int64_t share = share_of(in);
