@@ -4,9 +4,10 @@
 // smaller than the smallest normal fp32 number.
 //
 // Squares are summed in 64 bits: no finite fp32 or bf16 gradient overflows or
-// vanishes in its square, and 2^53 leaves the order of summation without
-// effect on the 32-bit result.  The order is fixed all the same (a block's
-// share, then the blocks in order), so equal inputs give equal bits.
+// vanishes in its square, and the sum loses 2^-40 of its size at most: the 32-bit
+// norm is the exact one rounded, or its neighbour where the exact one lies that
+// near to the middle of two.  The order of summation is fixed (a block's share, then the blocks in
+// order), so equal inputs give equal bits.
 #include "grad_clip.h"
 #include "int8.h"
 

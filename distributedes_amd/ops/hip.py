@@ -101,7 +101,9 @@ class HipOps:
 
     # --- 8-bit rows and products -----------------------------------------
     # No gradient passes through these: the framework estimates its gradients
-    # from forward passes.  An argument that requires one is refused.
+    # from forward passes.  An argument that requires one, or carries one of
+    # forward mode, is refused.  A write to `out` counts as a write for autograd.
+    # `out` overlaps no argument, unless said otherwise.
 
     def quantize_rows(self, x, out=None):
         """x [..., K] (fp32/bf16/fp16, K <= 131072) -> (codes [..., K] int8,
@@ -119,8 +121,10 @@ class HipOps:
 
     def int8_matmul(self, xq, sx, wq, sw, bias=None, activation="none",
                     out_dtype=torch.float32, out=None):
-        """act(sum_k xq[m, k] wq[n, k] * sx[m] * sw[n] + bias[n]): codes and
-        scales of quantize_rows on both sides, summed exactly in int32.
+        """act(sum_k xq[m, k] wq[n, k] * sx[m] * sw[n] + bias[n]): codes in
+        [-127, 127] and scales on both sides, as quantize_rows gives them; sums
+        are exact in int32, and their scaling stays in range wherever the result
+        does.
 
         One policy: xq [..., K] with wq [N, K] -> [..., N].  Members with
         weights of their own: xq [B, M, K] with wq [B, N, K] -> [B, M, N].
@@ -146,6 +150,7 @@ class HipOps:
         """-> ([t * c for t in tensors], norm), with c = max_norm / norm (fp64)
         where norm > max_norm, else 1; the norm stays on the GPU.  A NaN norm
         leaves the values as they are, an infinite one gives c = 0.
-        out: tensors to write to (the tensors themselves clip in place)."""
+        out: contiguous tensors to write to (the tensors themselves clip in
+        place)."""
         clipped, norm = self.ext2.clip_by_global_norm(tensors, max_norm, out)
         return (clipped if out is None else list(out)), norm
