@@ -2,7 +2,8 @@
 //
 // Every entry checks its arguments before it asks where the tensors live, so
 // that a wrong call is refused alike with and without a GPU (ops/reference.py
-// refuses the same); wrong values are ValueErrors.  Kernels run on the current stream of the tensors' own device,
+// refuses the same types, shapes, outputs and gradients); wrong values are
+// ValueErrors.  Kernels run on the current stream of the tensors' own device,
 // workspaces come from the caching allocator (and so belong to the graph, where
 // one is being captured), and no call waits for the GPU.
 #include <ATen/hip/HIPContext.h>
@@ -78,8 +79,8 @@ void check_place(const Tensor& t, const Tensor& like, const char* what) {
 void mark_written(const Tensor& t) { t.unsafeGetTensorImpl()->bump_version(); }
 
 // Kernels read memory as it is: a view that torch negates when it reads it is
-// written out first, and none is written to.  (resolve_neg alone goes through torch's
-// dispatcher where there is nothing to do, too.)
+// written out first, and none is written to.  (resolve_neg alone goes through
+// torch's dispatcher where there is nothing to do, too.)
 Tensor plain(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
 
 void check_plain(const Tensor& t, const char* what) {
